@@ -450,6 +450,35 @@ int lamq_attention_causal_bf16(const uint16_t* q, int64_t sqb, int64_t sqh, int6
                                int64_t Hkv, int64_t T, int64_t D, float scale, void* stream);
 
 /* ----------------------------------------------------------------------------------------------
+ * The attention of training (the student of finetune.py's distillation runs the same layers as the capture): the
+ * forward above over each sequence's own length, keeping what its backward needs, and the backward, which recomputes
+ * the probabilities. With S = scale q k^T over u <= t < len_b and P = exp(S - lse):
+ *   out = P v,  lse[b, h, t] = log sum_u exp(S_tu);   delta_t = sum_d dout_td out_td,  dS = P (dout v^T - delta),
+ *   dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout  (dk and dv summed over a key/value head's query heads)
+ *   q, dout, out, dq [B, H, T, 128], k, v, dk, dv [B, Hkv, T, 128] bf16 bits, each by its (batch, head, token)
+ *   strides in elements (lamq_heads), the head dim contiguous; strides multiples of 8, inputs 16-byte aligned, what
+ *   is written 8-byte aligned and none of it overlapping another tensor.
+ *   lse   [B, H, T] float32, written by the forward, read by the backward
+ *   lens  [B] int32 on the device, or NULL (all T): tokens past lens[b] (held to 0 .. T) are padding. Nothing is
+ *         read there; their rows of out and of the gradients are zeros, their lse -inf.
+ * Sums, scores and dP are float32; P and dS are rounded to bf16 as operands of the next product, each result once.
+ * The results do not depend on scheduling. Limits as lamq_attention_causal_bf16.
+ * ---------------------------------------------------------------------------------------------- */
+typedef struct {
+    uint16_t* data;
+    int64_t sb, sh, st;
+} lamq_heads;
+int lamq_attention_causal_lse_bf16(const lamq_heads* q, const lamq_heads* k, const lamq_heads* v, const lamq_heads* out,
+                                   float* lse, const int32_t* lens, int64_t B, int64_t H, int64_t Hkv, int64_t T,
+                                   int64_t D, float scale, void* stream);
+size_t lamq_attention_causal_grad_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t T);
+int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_heads* k, const lamq_heads* v, const lamq_heads* out,
+                                    const float* lse, const lamq_heads* dout, const int32_t* lens, const lamq_heads* dq,
+                                    const lamq_heads* dk, const lamq_heads* dv, int64_t B, int64_t H, int64_t Hkv,
+                                    int64_t T, int64_t D, float scale, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+
+/* ----------------------------------------------------------------------------------------------
  * Measurement only; no counterpart in the reference. The L2-to-CU delivery ceiling of the direct global->LDS load path
  * the Gram kernels feed their MFMAs through: `workgroups` workgroups (one a CU: 160 KB of LDS each) stream `stages`
  * stages of 32 KB each (1 KB loads of 16 bytes a lane, a five-buffer LDS ring, one barrier a stage) from the

@@ -75,6 +75,9 @@ SIGNATURES = {
                                          _c_flt, _p]),
     "lamq_attention_causal_bf16": (_c_int, [_p] + [_c_i64] * 3 + [_p] + [_c_i64] * 3 + [_p] + [_c_i64] * 3 + [_p]
                                    + [_c_i64] * 3 + [_c_i64] * 5 + [_c_flt, _p]),
+    "lamq_attention_causal_lse_bf16": (_c_int, [_p] * 6 + [_c_i64] * 5 + [_c_flt, _p]),
+    "lamq_attention_causal_grad_workspace_size": (_c_size, [_c_i64] * 4),
+    "lamq_attention_causal_grad_bf16": (_c_int, [_p] * 10 + [_c_i64] * 5 + [_c_flt, _p, _c_size, _p]),
     "lamq_probe_l2_delivery": (_c_int, [_p, _c_i64, _c_int, _c_int, _p]),
 }
 
@@ -97,6 +100,12 @@ class PackGroup(ctypes.Structure):
 
     _fields_ = [("src", _p), ("ld", _c_i64), ("src_rows", _c_i64), ("rows", _p), ("m", _c_i64), ("base", ctypes.c_int32),
                 ("k", _c_int), ("codes", _p), ("ldc", _c_i64)]
+
+
+class Heads(ctypes.Structure):
+    """lamq_heads of include/lamq.h: a [batch, head, token, head dim] tensor by its strides."""
+
+    _fields_ = [("data", _p), ("sb", _c_i64), ("sh", _c_i64), ("st", _c_i64)]
 
 
 _LIB = None

@@ -1,0 +1,396 @@
+// The backward pass of the causal grouped-query attention of training: the probabilities are recomputed from the
+// forward's log-sum-exp, tile by tile, and never reach memory.
+//
+// With S = scale Q K^T over u <= t < len, P = exp(S - lse), O = P V and dO the gradient of O:
+//   delta_t = sum_d dO_td O_td,  dP = dO V^T,  dS = P (dP - delta),
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,  dK and dV summed over a key/value head's query heads.
+//
+// Two kernels, so that each gradient has one owner and its sums one order (no atomics): attention_dq_kernel owns 128
+// queries and walks the keys up to them, forming S^T, dP^T and dQ^T += K^T dS^T; attention_dkdv_kernel owns 128 keys and
+// walks the query heads and queries from them on, forming S, dP, dV^T += dO^T P and dK^T += Q^T dS. Seven products where
+// five would do with one pass; the two formed twice cost less than a float32 dQ added up in memory (a read and a
+// write of 4 bytes per query, head dim and key block) and keep the results the same from run to run.
+//
+// The operand layouts are the forward's (32x32x16 bf16 MFMA): with the owned rows as columns of the result, S^T (or S)
+// and dP come out as the second product's B operand as they stand, and that product's A operand is the walked tile read
+// transposed (ds_read_b64_tr_b16) in the result's own order. A walked tile is read both ways, so its 16-byte chunks are
+// XOR-swizzled by at_f(row), the row's two low bit pairs exchanged: 16 rows at one chunk touch 16 different chunk
+// slots, and so do the four rows and four chunks a transposing read serves at once.
+//
+// P is rounded to bf16 for dV as the forward rounds it for O, dS to bf16 for dQ and dK, the operand type of the matrix
+// instructions; scores, dP, delta and every sum are float32, each gradient rounded once at its end.
+#include "attention.h"
+
+#define AG_R 32                       // rows a wave owns
+#define AG_W 64                       // rows of a walked block
+#define AG_OWN 128                    // rows a workgroup owns
+#define AG_OPB (AG_W * AT_D * 2)      // bytes of one operand's block (16 KB)
+
+__device__ __forceinline__ int at_f(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+__device__ __forceinline__ uint32_t at_fsw(int row, int chunk)
+{
+    return (uint32_t)(row * (AT_D * 2) + ((chunk ^ at_f(row)) << 4));
+}
+
+// A block of 64 rows r0 .. of an operand into LDS (global_load_lds, 16 bytes a lane): wave wv's instruction q fills rows
+// 16 wv + 4 q .. + 3, lane l the slot l % 16 of row 16 wv + 4 q + l / 16. Rows past `last` read row `last`.
+__device__ __forceinline__ void ag_load_block(const uint16_t* __restrict__ base, int64_t st, int r0, int last, int wv,
+                                              int lane, uint32_t buf)
+{
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int row = r0 + 16 * wv + 4 * q + (lane >> 4);
+        const int chunk = (lane & 15) ^ (((lane >> 4) << 2) | q);
+        load_lds16(base + (int64_t)(row < last ? row : last) * st + 8 * chunk, buf + (uint32_t)((4 * wv + q) * 1024));
+    }
+}
+
+// A operand of a product over the head dim: rows 32 hf + li, head dims 16 j + 8 hi .. + 7
+__device__ __forceinline__ lamq_at_bf16x8 ag_frag(const uint8_t* buf, int row, int j, int hi)
+{
+    return *reinterpret_cast<const lamq_at_bf16x8*>(buf + at_fsw(row, 2 * j + hi));
+}
+
+// A operand of a product over the walked rows: head dims 32 t + li, rows 32 hf + 16 mi + 4 hi + {0..3} and + 8
+__device__ __forceinline__ lamq_at_bf16x8 ag_tr_frag(uint32_t buf, int hf, int mi, int t, int lane)
+{
+    const int hi = lane >> 5, g = lane >> 4, i16 = lane & 15;
+    const int row = 32 * hf + 16 * mi + 4 * hi + (i16 >> 2);
+    const int col = 32 * t + 16 * (g & 1) + 4 * (i16 & 3);
+    const uint32_t a0 = buf + at_fsw(row, col >> 3) + 8 * ((col >> 2) & 1);
+    const uint32_t a1 = buf + at_fsw(row + 8, col >> 3) + 8 * ((col >> 2) & 1);
+    const lamq_at_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_at_lds_s4*)(uintptr_t)a0);
+    const lamq_at_s4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_at_lds_s4*)(uintptr_t)a1);
+    const short __attribute__((ext_vector_type(8))) w = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(lamq_at_bf16x8, w);
+}
+
+// eight consecutive head-dim values of a row
+__device__ __forceinline__ lamq_at_bf16x8 ag_row8(const uint16_t* p)
+{
+    return *reinterpret_cast<const lamq_at_bf16x8*>(p);
+}
+
+// the waits of the loads behind these fragments, before the loop whose own waits the compiler does not see
+__device__ __forceinline__ void ag_settle(lamq_at_bf16x8 (&f)[8])
+{
+    asm volatile("" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]), "+v"(f[4]), "+v"(f[5]), "+v"(f[6]), "+v"(f[7]));
+}
+
+// a transposed 128 x 32 result (four tiles: head dims 32 t + 8 r + 4 hi + {0..3} of the lane's row) times `scale`, as
+// bf16 (nearest, ties to even) into the row
+__device__ __forceinline__ void ag_store_row(uint16_t* row, const lamq_at_f32x16 (&acc)[4], float scale, int hi)
+{
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            uint32_t w2[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const __bf16 x0 = (__bf16)(acc[t][4 * r + 2 * e] * scale);
+                const __bf16 x1 = (__bf16)(acc[t][4 * r + 2 * e + 1] * scale);
+                w2[e] = (uint32_t)__builtin_bit_cast(uint16_t, x0) | ((uint32_t)__builtin_bit_cast(uint16_t, x1) << 16);
+            }
+            *reinterpret_cast<uint2*>(row + 32 * t + 8 * r + 4 * hi) = make_uint2(w2[0], w2[1]);
+        }
+}
+
+// workgroup -> (pair of sequence and key/value head, index in the pair's `per`): the pairs spread over the XCDs, so that
+// those that read the same keys and values run on one XCD together. False past the last workgroup.
+__device__ __forceinline__ bool ag_place(int pairs, int per, int& pair, int& rem)
+{
+    const int id = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+    if ((unsigned)id >= (unsigned)pairs * (unsigned)per) return false;
+    if (pairs % LAMQ_XCDS == 0) {
+        const int y = id / LAMQ_XCDS;
+        pair = y / per * LAMQ_XCDS + id % LAMQ_XCDS;
+        rem = y % per;
+    } else {
+        pair = id / per;
+        rem = id % per;
+    }
+    return true;
+}
+
+// dQ, and per query the log-sum-exp in units of log 2 and delta for the other kernel (rows [B, H, T] of stats and
+// stats + B H T).
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_dq_kernel(
+    AtView Q, AtView K, AtView V, AtView O, AtView dO, AtOut dQ, const float* __restrict__ lse,
+    const int32_t* __restrict__ lens, float* __restrict__ stats, int64_t nstats, int rep, int Hkv, int pairs, int Tall,
+    float scale, float scale_log2)
+{
+    __shared__ __align__(16) uint8_t lds[2][2][AG_OPB];  // [buffer][K, V]
+    const int nqb = (Tall + AG_OWN - 1) / AG_OWN;
+    int pair, rem;
+    if (!ag_place(pairs, nqb * rep, pair, rem)) return;
+    const int qb = nqb - 1 - rem / rep;  // the longest query blocks first
+    const int b = pair / Hkv, hk = pair % Hkv, h = hk * rep + rem % rep;
+    const int lane = (int)(threadIdx.x & 63), wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int li = lane & 31, hi = lane >> 5;
+    const int T = at_length(lens, b, Tall);
+    uint16_t* dQp = dQ.p + b * dQ.sb + (int64_t)h * dQ.sh;
+    const int own0 = qb * AG_OWN, own1 = own0 + AG_OWN < Tall ? own0 + AG_OWN : Tall;
+    if (own1 > T) {
+        at_zero_rows(dQp, dQ.st, own0 > T ? own0 : T, own1);
+        if (own0 >= T) return;  // uniform, before any barrier
+    }
+    const int q0 = own0 + AG_R * wv, myq = q0 + li, qrow = myq < T ? myq : T - 1;
+    const uint16_t* Kp = K.p + b * K.sb + (int64_t)hk * K.sh;
+    const uint16_t* Vp = V.p + b * V.sb + (int64_t)hk * V.sh;
+    const uint32_t base = lds_addr(lds);
+    const int wg_last = (own1 < T ? own1 : T) - 1;
+    const int nblk = wg_last / AG_W + 1;
+    const int my_last = q0 < T ? (q0 + AG_R < T ? q0 + AG_R : T) - 1 : -1;
+    auto load_block = [&](int kb) {
+        const uint32_t buf = base + (uint32_t)((kb & 1) * 2 * AG_OPB);
+        ag_load_block(Kp, K.st, kb * AG_W, T - 1, wv, lane, buf);
+        ag_load_block(Vp, V.st, kb * AG_W, T - 1, wv, lane, buf + AG_OPB);
+    };
+    load_block(0);
+    lamq_at_bf16x8 qf[8], df[8];
+    float delta = 0.0f, lse2;
+    {
+        const uint16_t* Qr = Q.p + b * Q.sb + (int64_t)h * Q.sh + (int64_t)qrow * Q.st + 8 * hi;
+        const uint16_t* Dr = dO.p + b * dO.sb + (int64_t)h * dO.sh + (int64_t)qrow * dO.st + 8 * hi;
+        const uint16_t* Or = O.p + b * O.sb + (int64_t)h * O.sh + (int64_t)qrow * O.st + 8 * hi;
+        lamq_at_bf16x8 of[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            qf[j] = ag_row8(Qr + 16 * j);
+            df[j] = ag_row8(Dr + 16 * j);
+            of[j] = ag_row8(Or + 16 * j);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) delta = fmaf((float)df[j][e], (float)of[j][e], delta);
+        delta = at_sum32(delta);
+        const int64_t at = ((int64_t)b * Hkv * rep + h) * Tall + qrow;
+        lse2 = lse[at] * AT_LOG2E;
+        if (hi == 0 && myq < T) {
+            stats[at] = lse2;
+            stats[nstats + at] = delta;
+        }
+    }
+    ag_settle(qf);
+    ag_settle(df);
+    lamq_at_f32x16 acc[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[t][v] = 0.0f;
+    for (int kb = 0; kb < nblk; ++kb) {
+        wait_vm<0>();     // this wave's loads of block kb have landed
+        __syncthreads();  // everyone's; the other buffer is free
+        if (kb + 1 < nblk) load_block(kb + 1);
+        const int k0 = kb * AG_W;
+        const uint8_t* kl = lds[kb & 1][0];
+        const uint8_t* vl = lds[kb & 1][1];
+        const uint32_t kbase = base + (uint32_t)((kb & 1) * 2 * AG_OPB);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            if (k0 + 32 * hf > my_last) continue;  // uniform: past this wave's queries
+            lamq_at_f32x16 s, dp;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                s[v] = 0.0f;
+                dp[v] = -delta;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(kl, 32 * hf + li, j, hi), qf[j], s, 0, 0, 0);
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(vl, 32 * hf + li, j, hi), df[j], dp, 0, 0, 0);
+            }
+            if (k0 + 32 * hf + 31 > q0) {  // the causal mask, only where the half reaches past the wave's first query
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    s[v] = k0 + 32 * hf + 8 * (v >> 2) + 4 * hi + (v & 3) <= myq ? s[v] : -__builtin_inff();
+            }
+            lamq_at_bf16x8 dsf[2];
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                dsf[v >> 3][v & 7] = (__bf16)(__builtin_amdgcn_exp2f(fmaf(s[v], scale_log2, -lse2)) * dp[v]);
+#pragma unroll
+            for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(kbase, hf, mi, t, lane), dsf[mi], acc[t],
+                                                                     0, 0, 0);
+        }
+    }
+    if (myq < T) ag_store_row(dQp + (int64_t)myq * dQ.st, acc, scale, hi);
+}
+
+// dK and dV of 128 keys of a key/value head, over its query heads and the queries from the keys on.
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_dkdv_kernel(
+    AtView Q, AtView K, AtView V, AtView dO, AtOut dK, AtOut dV, const int32_t* __restrict__ lens,
+    const float* __restrict__ stats, int64_t nstats, int rep, int Hkv, int pairs, int Tall, float scale, float scale_log2)
+{
+    __shared__ __align__(16) uint8_t lds[2][2][AG_OPB];  // [buffer][Q, dO]
+    __shared__ __align__(16) float row_stats[2][2][AG_W];  // [buffer][lse, delta]
+    const int nkb = (Tall + AG_OWN - 1) / AG_OWN;
+    int pair, kb;
+    if (!ag_place(pairs, nkb, pair, kb)) return;  // the first keys have the most queries: they go out first
+    const int b = pair / Hkv, hk = pair % Hkv;
+    const int lane = (int)(threadIdx.x & 63), wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int li = lane & 31, hi = lane >> 5;
+    const int T = at_length(lens, b, Tall);
+    uint16_t* dKp = dK.p + b * dK.sb + (int64_t)hk * dK.sh;
+    uint16_t* dVp = dV.p + b * dV.sb + (int64_t)hk * dV.sh;
+    const int own0 = kb * AG_OWN, own1 = own0 + AG_OWN < Tall ? own0 + AG_OWN : Tall;
+    if (own1 > T) {
+        const int first = own0 > T ? own0 : T;
+        at_zero_rows(dKp, dK.st, first, own1);
+        at_zero_rows(dVp, dV.st, first, own1);
+        if (own0 >= T) return;  // uniform, before any barrier
+    }
+    const int k0 = own0 + AG_R * wv, myk = k0 + li, krow = myk < T ? myk : T - 1;
+    const uint32_t base = lds_addr(lds), sbase = lds_addr(row_stats);
+    const int b0 = own0 / AG_W, nblk = (T - 1) / AG_W - b0 + 1, items = rep * nblk;
+    auto load_block = [&](int it) {
+        const int h = hk * rep + it / nblk, r0 = (b0 + it % nblk) * AG_W;
+        const uint32_t buf = base + (uint32_t)((it & 1) * 2 * AG_OPB);
+        ag_load_block(Q.p + b * Q.sb + (int64_t)h * Q.sh, Q.st, r0, T - 1, wv, lane, buf);
+        ag_load_block(dO.p + b * dO.sb + (int64_t)h * dO.sh, dO.st, r0, T - 1, wv, lane, buf + AG_OPB);
+        if (wv < 2) {
+            const int row = r0 + lane < T ? r0 + lane : T - 1;
+            load_lds4(stats + wv * nstats + ((int64_t)b * Hkv * rep + h) * Tall + row,
+                      sbase + (uint32_t)(((it & 1) * 2 + wv) * AG_W * 4));
+        }
+    };
+    load_block(0);
+    lamq_at_bf16x8 kf[8], vf[8];
+    {
+        const uint16_t* Kr = K.p + b * K.sb + (int64_t)hk * K.sh + (int64_t)krow * K.st + 8 * hi;
+        const uint16_t* Vr = V.p + b * V.sb + (int64_t)hk * V.sh + (int64_t)krow * V.st + 8 * hi;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            kf[j] = ag_row8(Kr + 16 * j);
+            vf[j] = ag_row8(Vr + 16 * j);
+        }
+    }
+    ag_settle(kf);
+    ag_settle(vf);
+    lamq_at_f32x16 dk[4], dv[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) dk[t][v] = dv[t][v] = 0.0f;
+    for (int it = 0; it < items; ++it) {
+        wait_vm<0>();     // this wave's loads of the block have landed
+        __syncthreads();  // everyone's; the other buffer is free
+        if (it + 1 < items) load_block(it + 1);
+        const int r0 = (b0 + it % nblk) * AG_W;
+        const uint8_t* ql = lds[it & 1][0];
+        const uint8_t* dl = lds[it & 1][1];
+        const uint32_t qbase = base + (uint32_t)((it & 1) * 2 * AG_OPB), dbase = qbase + AG_OPB;
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) {
+            const int q0 = r0 + 32 * hf;
+            if (q0 + 31 < k0 || q0 >= T) continue;  // uniform: no query here sees this wave's keys
+            const float* sl = &row_stats[it & 1][0][32 * hf + 4 * hi];
+            lamq_at_f32x16 s, dp;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float4 dl4 = *reinterpret_cast<const float4*>(sl + AG_W + 8 * r);
+                dp[4 * r] = -dl4.x;
+                dp[4 * r + 1] = -dl4.y;
+                dp[4 * r + 2] = -dl4.z;
+                dp[4 * r + 3] = -dl4.w;
+            }
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(ql, 32 * hf + li, j, hi), kf[j], s, 0, 0, 0);
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(dl, 32 * hf + li, j, hi), vf[j], dp, 0, 0, 0);
+            }
+            if (q0 < k0 + 31 || q0 + 31 >= T) {  // the causal mask and the queries past the length
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int q = q0 + 8 * (v >> 2) + 4 * hi + (v & 3);
+                    s[v] = myk <= q && q < T ? s[v] : -__builtin_inff();
+                }
+            }
+            lamq_at_bf16x8 pf[2], dsf[2];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float4 ls4 = *reinterpret_cast<const float4*>(sl + 8 * r);
+                const float ls[4] = {ls4.x, ls4.y, ls4.z, ls4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int v = 4 * r + e;
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[v], scale_log2, -ls[e]));
+                    pf[v >> 3][v & 7] = (__bf16)p;
+                    dsf[v >> 3][v & 7] = (__bf16)(p * dp[v]);
+                }
+            }
+#pragma unroll
+            for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    dv[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(dbase, hf, mi, t, lane), pf[mi], dv[t], 0, 0,
+                                                                    0);
+                    dk[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(qbase, hf, mi, t, lane), dsf[mi], dk[t], 0,
+                                                                    0, 0);
+                }
+        }
+    }
+    if (myk < T) {
+        ag_store_row(dKp + (int64_t)myk * dK.st, dk, scale, hi);
+        ag_store_row(dVp + (int64_t)myk * dV.st, dv, 1.0f, hi);
+    }
+}
+
+extern "C" size_t lamq_attention_causal_grad_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t T)
+{
+    if (B < 1 || H < 1 || Hkv < 1 || T < 1) return 0;
+    return (size_t)B * H * T * 2 * sizeof(float);
+}
+
+extern "C" int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_heads* k, const lamq_heads* v,
+                                               const lamq_heads* out, const float* lse, const lamq_heads* dout,
+                                               const int32_t* lens, const lamq_heads* dq, const lamq_heads* dk,
+                                               const lamq_heads* dv, int64_t B, int64_t H, int64_t Hkv, int64_t T,
+                                               int64_t D, float scale, void* workspace, size_t workspace_bytes,
+                                               void* stream)
+{
+    if (!q || !k || !v || !out || !lse || !dout || !dq || !dk || !dv) return LAMQ_EINVAL;
+    if (B < 0 || H < 1 || Hkv < 1 || T < 0 || H % Hkv != 0) return LAMQ_EINVAL;
+    if (D != AT_D) return LAMQ_EUNSUP;
+    if (!(scale > 0.0f) || !(scale < 3.0e38f)) return LAMQ_EINVAL;
+    const lamq_heads* all[8] = {q, k, v, out, dout, dq, dk, dv};
+    for (int i = 0; i < 8; ++i) {
+        const lamq_heads& x = *all[i];
+        if (!x.data || (uintptr_t)x.data % (i < 5 ? 16 : 8)) return LAMQ_EINVAL;  // 16-byte loads, 8-byte stores
+        for (int64_t s : {x.sb, x.sh, x.st})
+            if (s < 0 || s % 8 != 0) return LAMQ_EINVAL;
+    }
+    if (B == 0 || T == 0) return LAMQ_OK;
+    if (B > 65535 || H > 65535 || T > 0x7fffff) return LAMQ_EUNSUP;
+    const int64_t qwgs = cdiv(T, AG_OWN) * H * B, kwgs = cdiv(T, AG_OWN) * Hkv * B;
+    if (qwgs > 0x7fffffff) return LAMQ_EUNSUP;
+    if (!workspace || (uintptr_t)workspace % 4 ||
+        workspace_bytes < lamq_attention_causal_grad_workspace_size(B, H, Hkv, T))
+        return LAMQ_EINVAL;
+    const AtView vq{q->data, q->sb, q->sh, q->st}, vk{k->data, k->sb, k->sh, k->st}, vv{v->data, v->sb, v->sh, v->st},
+        vo{out->data, out->sb, out->sh, out->st}, vd{dout->data, dout->sb, dout->sh, dout->st};
+    const AtOut oq{dq->data, dq->sb, dq->sh, dq->st}, ok{dk->data, dk->sb, dk->sh, dk->st},
+        ov{dv->data, dv->sb, dv->sh, dv->st};
+    float* stats = reinterpret_cast<float*>(workspace);
+    const int64_t nstats = B * H * T;
+    hipStream_t s = as_stream(stream);
+    // a grid's work items along x must stay below 2^32, so past 2^22 workgroups they go out in rows
+    auto grid = [](int64_t wgs) {
+        const int64_t gx = wgs < AT_GRID_X ? wgs : AT_GRID_X;
+        return dim3((unsigned)gx, (unsigned)cdiv(wgs, gx));
+    };
+    hipLaunchKernelGGL(attention_dq_kernel, grid(qwgs), dim3(256), 0, s, vq, vk, vv, vo, vd, oq, lse, lens, stats, nstats,
+                       (int)(H / Hkv), (int)Hkv, (int)(B * Hkv), (int)T, scale, scale * AT_LOG2E);
+    LAMQ_LAUNCH_CHECK();
+    hipLaunchKernelGGL(attention_dkdv_kernel, grid(kwgs), dim3(256), 0, s, vq, vk, vv, vd, ok, ov, lens, stats, nstats,
+                       (int)(H / Hkv), (int)Hkv, (int)(B * Hkv), (int)T, scale, scale * AT_LOG2E);
+    LAMQ_LAUNCH_CHECK();
+    return LAMQ_OK;
+}

@@ -643,6 +643,80 @@ def attention_causal(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     return out
 
 
+def _heads(t: torch.Tensor) -> int:
+    """t [B, heads, T, D] as a lamq_heads argument (an address ctypes keeps alive for the call)."""
+    return ctypes.byref(_abi.Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)))
+
+
+def _need_heads(t, shape, name: str):
+    need(t, torch.bfloat16, name, 4)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}")
+
+
+def _attention_shapes(q, k, v, lens):
+    need(q, torch.bfloat16, "q", 4)
+    need(k, torch.bfloat16, "k", 4)
+    B, H, T, D = q.shape
+    Hkv = k.shape[1]
+    if H < 1 or Hkv < 1 or H % Hkv or tuple(k.shape) != (B, Hkv, T, D):
+        raise ValueError("k and v must be [B, Hkv, T, D] with Hkv dividing q's heads")
+    _need_heads(v, k.shape, "v")
+    if lens is not None:
+        need(lens, torch.int32, "lens", 1)
+        if lens.numel() != B:
+            raise ValueError("one length per sequence")
+    devs = {t.device for t in (q, k, v) + (() if lens is None else (lens,))}
+    if len(devs) != 1:
+        raise ValueError("all tensors must be on one device")
+    return B, H, Hkv, T, D
+
+
+def _by_token(B: int, heads: int, T: int, like: torch.Tensor) -> torch.Tensor:
+    """An empty [B, heads, T, D] tensor in the layers' [B, T, heads, D] layout."""
+    return torch.empty(B, T, heads, like.shape[3], dtype=like.dtype, device=like.device).transpose(1, 2)
+
+
+def attention_causal_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
+                         lens: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The attention of training (lamq_attention_causal_lse_bf16): attention_causal over the first lens[b] tokens of
+    each sequence (int32 [B] on the device, held to 0 .. T; None: all T), and the log-sum-exp of every query's scaled
+    scores, which attention_causal_grad takes. Returns (out [B, H, T, 128] bf16, a view of a [B, T, H, 128] buffer,
+    lse [B, H, T] float32); tokens past a length have out 0 and lse -inf, and nothing is read there."""
+    B, H, Hkv, T, D = _attention_shapes(q, k, v, lens)
+    out = _by_token(B, H, T, q)
+    lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device)
+    if B and T:
+        check(lib().lamq_attention_causal_lse_bf16(_heads(q), _heads(k), _heads(v), _heads(out), ptr(lse), ptr(lens), B,
+                                                   H, Hkv, T, D, float(scale), stream(q.device)),
+              "attention_causal_lse")
+    return out, lse
+
+
+def attention_causal_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                          lse: torch.Tensor, scale: float, lens: torch.Tensor | None = None) -> tuple:
+    """The gradients of attention_causal_lse (lamq_attention_causal_grad_bf16) for the gradient dout of its out: (dq
+    [B, H, T, 128], dk, dv [B, Hkv, T, 128]) bf16, views of [B, T, heads, 128] buffers, zero past a length. out and lse
+    are the forward's, scale and lens the ones it was given."""
+    B, H, Hkv, T, D = _attention_shapes(q, k, v, lens)
+    _need_heads(dout, q.shape, "dout")
+    _need_heads(out, q.shape, "out")
+    need(lse, torch.float32, "lse", 3)
+    if tuple(lse.shape) != (B, H, T) or not lse.is_contiguous():
+        raise ValueError("lse must be a contiguous [B, H, T]")
+    if {dout.device, out.device, lse.device} != {q.device}:
+        raise ValueError("all tensors must be on one device")
+    dq, dk, dv = _by_token(B, H, T, q), _by_token(B, Hkv, T, q), _by_token(B, Hkv, T, q)
+    if B and T:
+        nbytes = lib().lamq_attention_causal_grad_workspace_size(B, H, Hkv, T)
+        ws = workspace(nbytes, q.device)
+        check(lib().lamq_attention_causal_grad_bf16(_heads(q), _heads(k), _heads(v), _heads(out), ptr(lse),
+                                                    _heads(dout), ptr(lens), _heads(dq), _heads(dk), _heads(dv), B, H,
+                                                    Hkv, T, D, float(scale), ptr(ws), nbytes, stream(q.device)),
+              "attention_causal_grad")
+    return dq, dk, dv
+
+
 class EventLog(dict):
     """key -> list of (start, end) torch.cuda.Event pairs. lead_cycles > 0: before each span's start event, a GPU spin
     of that many cycles (torch.cuda._sleep) keeps the stream busy while the host enqueues the span, so that a span

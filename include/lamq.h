@@ -341,6 +341,26 @@ int lamq_kl_rows_noalloc(const uint16_t* ref, const uint16_t* q, int64_t T, int6
                          const float* w, float* kl, double* sums, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * The KL loss of distillation with its gradient (the loss finetune.py descends; the KL of compiler.py:177-188):
+ *   kl_t = sum_v softmax(ref_t)_v (log_softmax(ref_t)_v - log_softmax(q_t)_v)
+ *   loss = sum_t w_t kl_t / sum_t w_t,   grad_t = w_t / sum(w) (softmax(q_t) - softmax(ref_t))
+ *   ref, q  [T, V] bf16 (lamq_kl_rows_grad) or float32 (_f32), row strides ldr, ldq, rows at any element alignment
+ *   w       [T] float32 or NULL (all 1). A row of weight 0 is left out: kl 0, gradient 0, its logits not read; the
+ *           loss is NaN if every row is left out
+ *   kl      [T] float32; loss [1] float32; grad [T, V] in the logits' type, row stride ldg, not overlapping them
+ * A logit of -inf has probability 0; kl is +inf where ref is finite and q is not, and a row with no finite logit gives
+ * NaN. Sums are float64, in a fixed order. T <= 16,777,215 (LAMQ_EUNSUP above). workspace: 16-byte aligned,
+ * lamq_kl_rows_grad_workspace_size(T, V) bytes.
+ * ---------------------------------------------------------------------------------------------- */
+size_t lamq_kl_rows_grad_workspace_size(int64_t T, int64_t V);
+int lamq_kl_rows_grad(const uint16_t* ref, const uint16_t* q, int64_t T, int64_t V, int64_t ldr, int64_t ldq,
+                      const float* w, float* kl, float* loss, uint16_t* grad, int64_t ldg, void* workspace,
+                      size_t workspace_bytes, void* stream);
+int lamq_kl_rows_grad_f32(const float* ref, const float* q, int64_t T, int64_t V, int64_t ldr, int64_t ldq,
+                          const float* w, float* kl, float* loss, float* grad, int64_t ldg, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Pack row-trellis states into the opgraph-packed-1 bitstream.
  * Replaces compiler_artifact.py:225-240 (pack_symbols) and :261-284 (valid_path, pack_trellis):
  *   symbols = state & (2^k - 1), each row padded forward to a multiple of 32, reversed, then

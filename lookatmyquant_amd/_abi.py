@@ -61,6 +61,9 @@ SIGNATURES = {
     "lamq_kl_rows": (_c_int, [_p, _p, _c_i64, _c_i64, _c_i64, _c_i64, _p, _p, _p, _p, _c_size, _p]),
     "lamq_kl_rows_f32": (_c_int, [_p, _p, _c_i64, _c_i64, _c_i64, _c_i64, _p, _p, _p, _p, _c_size, _p]),
     "lamq_kl_rows_noalloc": (_c_int, [_p, _p, _c_i64, _c_i64, _c_i64, _c_i64, _p, _p, _p, _p]),
+    "lamq_kl_rows_grad_workspace_size": (_c_size, [_c_i64] * 2),
+    "lamq_kl_rows_grad": (_c_int, [_p] * 2 + [_c_i64] * 4 + [_p] * 4 + [_c_i64, _p, _c_size, _p]),
+    "lamq_kl_rows_grad_f32": (_c_int, [_p] * 2 + [_c_i64] * 4 + [_p] * 4 + [_c_i64, _p, _c_size, _p]),
     "lamq_pack_trellis": (_c_int, [_p, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _p, _c_i64, _p, _p]),
     "lamq_pack_codes": (_c_int, [_p, _c_i64, _c_i64, _p, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _p, _c_i64, _p, _p]),
     "lamq_pack_codes_groups": (_c_int, [_p, _c_int, _c_i64, _c_int, _c_int, _p, _p]),

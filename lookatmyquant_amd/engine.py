@@ -1115,6 +1115,42 @@ def kl_rows_noalloc(ref: torch.Tensor, q: torch.Tensor, kl: torch.Tensor, sums: 
     return kl, sums
 
 
+def kl_rows_grad(ref: torch.Tensor, q: torch.Tensor, w: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The KL loss of distillation with its gradient (lamq_kl_rows_grad): for reference and student logits [T, V],
+    both bf16 or both float32, and token weights w [T] (None: all 1), (kl [T] float32, loss = sum w kl / sum w, a float32
+    scalar on the device, grad [T, V] = d loss / d q in the logits' type, written into `out` if given). A row of weight
+    0 is left out: kl and gradient 0, its logits not read. Nothing synchronises."""
+    dt = ref.dtype if ref.dtype in (torch.bfloat16, torch.float32) else torch.bfloat16
+    need(ref, dt, "ref", 2)
+    need(q, dt, "q", 2)
+    if ref.shape != q.shape or ref.shape[1] < 1:
+        raise ValueError("ref and q must have the same shape [T, V]")
+    T, V = ref.shape
+    wv = None
+    if w is not None:
+        if w.numel() != T:
+            raise ValueError("one weight per token")
+        wv = w.reshape(-1).to(device=ref.device, dtype=torch.float32).contiguous()
+    if out is None:
+        out = torch.empty(T, V, dtype=dt, device=ref.device)
+    need(out, dt, "out", 2)
+    if out.shape != ref.shape or len({ref.device, q.device, out.device}) != 1:
+        raise ValueError("out must be [T, V], all tensors on one device")
+    kl = torch.empty(T, dtype=torch.float32, device=ref.device)
+    if T == 0:
+        return kl, torch.full((), float("nan"), device=ref.device), out
+    loss = torch.empty((), dtype=torch.float32, device=ref.device)
+    nbytes = lib().lamq_kl_rows_grad_workspace_size(T, V)
+    ws = workspace(nbytes, ref.device)
+    fn = lib().lamq_kl_rows_grad if dt == torch.bfloat16 else lib().lamq_kl_rows_grad_f32
+    # the stride of a single row is not its length in general, and need not be
+    step = lambda t: t.stride(0) if T > 1 else V
+    check(fn(ptr(ref), ptr(q), T, V, step(ref), step(q), ptr(wv), ptr(kl), ptr(loss), ptr(out), step(out), ptr(ws), nbytes,
+             stream(ref.device)), "kl_rows_grad")
+    return kl, loss, out
+
+
 # ----------------------------------------------------------------------------- packing (compiler_artifact.py:276-284)
 
 

@@ -499,6 +499,25 @@ int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_heads* k, co
                                     void* stream);
 
 /* ----------------------------------------------------------------------------------------------
+ * Orthogonalisation of a weight matrix's update by Newton-Schulz products (the update of the distillation step; no
+ * counterpart in the reference): for each matrix G of a batch,
+ *   X = G / ||G||_F;  steps times: A = X X^T, B = b A + c A^2, X = a X + B X  (on the short side);  out = bf16(X)
+ *   G     [batch][rows, cols] bf16 bits or float32, row stride ld >= cols, matrix stride `stride` (0: one for all)
+ *   out   [batch][rows, cols] bf16 bits, row stride ldo >= cols, matrix stride so >= rows ldo, not overlapping G
+ * A zero matrix gives zeros, one with a NaN or an infinity NaN. The products take float16 operands (X as a sum of two)
+ * and float32 sums; X's singular values, which a step maps to a s + b s^3 + c s^5, must stay within 8 from any start
+ * in [0, 1], or LAMQ_EINVAL. rows, cols <= 2^20, batch <= 65,535 (LAMQ_EUNSUP above). workspace: 16-byte aligned,
+ * lamq_orthogonalize_workspace_size(batch, rows, cols) bytes.
+ * ---------------------------------------------------------------------------------------------- */
+size_t lamq_orthogonalize_workspace_size(int64_t batch, int64_t rows, int64_t cols);
+int lamq_orthogonalize_bf16(const uint16_t* G, int64_t batch, int64_t rows, int64_t cols, int64_t ld, int64_t stride,
+                            int steps, float a, float b, float c, uint16_t* out, int64_t ldo, int64_t so,
+                            void* workspace, size_t workspace_bytes, void* stream);
+int lamq_orthogonalize_f32(const float* G, int64_t batch, int64_t rows, int64_t cols, int64_t ld, int64_t stride,
+                           int steps, float a, float b, float c, uint16_t* out, int64_t ldo, int64_t so,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* ----------------------------------------------------------------------------------------------
  * Measurement only; no counterpart in the reference. The L2-to-CU delivery ceiling of the direct global->LDS load path
  * the Gram kernels feed their MFMAs through: `workgroups` workgroups (one a CU: 160 KB of LDS each) stream `stages`
  * stages of 32 KB each (1 KB loads of 16 bytes a lane, a five-buffer LDS ring, one barrier a stage) from the

@@ -81,6 +81,9 @@ SIGNATURES = {
     "lamq_attention_causal_lse_bf16": (_c_int, [_p] * 6 + [_c_i64] * 5 + [_c_flt, _p]),
     "lamq_attention_causal_grad_workspace_size": (_c_size, [_c_i64] * 4),
     "lamq_attention_causal_grad_bf16": (_c_int, [_p] * 10 + [_c_i64] * 5 + [_c_flt, _p, _c_size, _p]),
+    "lamq_orthogonalize_workspace_size": (_c_size, [_c_i64] * 3),
+    "lamq_orthogonalize_bf16": (_c_int, [_p] + [_c_i64] * 5 + [_c_int] + [_c_flt] * 3 + [_p, _c_i64, _c_i64, _p, _c_size, _p]),
+    "lamq_orthogonalize_f32": (_c_int, [_p] + [_c_i64] * 5 + [_c_int] + [_c_flt] * 3 + [_p, _c_i64, _c_i64, _p, _c_size, _p]),
     "lamq_probe_l2_delivery": (_c_int, [_p, _c_i64, _c_int, _c_int, _p]),
 }
 

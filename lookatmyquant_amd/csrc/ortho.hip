@@ -1,0 +1,428 @@
+// Orthogonalisation of a weight matrix's update by Newton-Schulz products: the step of an optimiser that moves a matrix
+// along the nearest semi-orthogonal matrix to its (averaged) gradient G,
+//   X = G / ||G||_F;  `steps` times:  A = X X^T,  B = b A + c A^2,  X = a X + B X,
+// X taken with its short side as rows (m <= n; a tall G transposed). Each step maps every singular value s of X to
+// a s + b s^3 + c s^5 and leaves the singular vectors alone.
+//
+// All three products run on v_mfma_f32_32x32x16_f16. float16 and not bf16: every matrix here is bounded (singular
+// values stay near 1 or below, checked on the host for the coefficients given), so bf16's range buys nothing and its
+// three bits fewer cost: on a gradient with a few strong directions the bf16 iteration ends 3e-2 from the exact one,
+// float16 4e-3. X is held as two float16 parts, X = hi + lo (22 bits): the products read hi, and a X, the term that
+// carries the small singular values, takes both, so a rounding of X is not multiplied by a in every step: 1e-3 and
+// below. All sums are float32. X, A and B are stored times 2^10 (exact), which keeps entries of 1e-4, as a normalised
+// large matrix has, clear of float16's smallest normal number; the largest entries, below 8, stay below 2^13.
+//
+// A and B are symmetric: only the tiles on and below the diagonal are computed and each is stored twice. Sizes are
+// padded with zeros to tiles, which changes no entry of any product.
+#include "common.h"
+
+#include <math.h>
+
+typedef _Float16 lamq_ns_f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 lamq_ns_f16x4 __attribute__((ext_vector_type(4)));
+typedef float lamq_ns_f32x16 __attribute__((ext_vector_type(16)));
+typedef short lamq_ns_s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) lamq_ns_s4 lamq_ns_lds_s4;
+
+#define NS_T 128                     // output tile
+#define NS_K 64                      // depth of a stage
+#define NS_OPB (NS_T * NS_K * 2)     // bytes of one operand's stage (16 KB)
+#define NS_PARTS 256                 // partial sums of squares a matrix
+#define NS_SCALE 1024.0f             // what X, A and B are stored times
+#define NS_UNSCALE (1.0f / 1024.0f)
+
+__device__ __forceinline__ float ns_load(const float* p) { return *p; }
+__device__ __forceinline__ float ns_load(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
+
+// The sum over the workgroup of 256, in every thread, in a fixed order.
+__device__ __forceinline__ double ns_sum(double x)
+{
+    __shared__ double s[4];
+    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
+    __syncthreads();
+    x = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    return x;
+}
+
+// float64 partial sums of squares of each matrix: float32 squares of a gradient can underflow or overflow
+template <typename Elt>
+__global__ __launch_bounds__(256) void ns_norm_kernel(const Elt* __restrict__ G, int64_t rows, int64_t cols, int64_t ld,
+                                                      int64_t stride, double* __restrict__ parts)
+{
+    const Elt* g = G + blockIdx.y * stride;
+    double x = 0.0;
+    const int64_t n = rows * cols;
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += 256 * (int64_t)gridDim.x) {
+        const double v = (double)ns_load(g + i / cols * ld + i % cols);
+        x += v * v;
+    }
+    x = ns_sum(x);
+    if (threadIdx.x == 0) parts[blockIdx.y * gridDim.x + blockIdx.x] = x;
+}
+
+// X = G / ||G|| (0 for a zero matrix) as hi + lo float16 parts, times 2^10, [mp][np] with zeros past G; a tall G
+// transposed. A workgroup takes 64 x 64 entries of X.
+template <typename Elt, bool TALL>
+__global__ __launch_bounds__(256) void ns_start_kernel(const Elt* __restrict__ G, int64_t rows, int64_t cols, int64_t ld,
+                                                       int64_t stride, const double* __restrict__ parts, int nparts,
+                                                       int mp, int np, uint16_t* __restrict__ hi,
+                                                       uint16_t* __restrict__ lo)
+{
+    __shared__ float tile[64][65];
+    const int64_t batch = blockIdx.z;
+    const double ss = ns_sum((int)threadIdx.x < nparts ? parts[batch * nparts + threadIdx.x] : 0.0);
+    const double f = ss > 0.0 ? (double)NS_SCALE / sqrt(ss) : ss;  // NaN stays
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+    const int x = threadIdx.x & 63;
+    const Elt* g = G + batch * stride;
+#pragma unroll 4
+    for (int y = threadIdx.x >> 6; y < 64; y += 4) {
+        // the tile in G's own order: along its rows
+        const int64_t r = (TALL ? c0 : r0) + y, c = (TALL ? r0 : c0) + x;
+        const float v = r < rows && c < cols ? (float)((double)ns_load(g + r * ld + c) * f) : 0.0f;
+        if (TALL)
+            tile[x][y] = v;
+        else
+            tile[y][x] = v;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int y = threadIdx.x >> 6; y < 64; y += 4) {
+        const float v = tile[y][x];
+        const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
+        const int64_t at = batch * mp * np + (int64_t)(r0 + y) * np + c0 + x;
+        hi[at] = __builtin_bit_cast(uint16_t, h);
+        lo[at] = __builtin_bit_cast(uint16_t, l);
+    }
+}
+
+// One stage of an operand whose rows run along the product's depth: 128 rows of 64, 128 bytes a row in LDS, 16-byte
+// chunks XOR-swizzled by row / 2 % 8 (16 rows at one chunk then touch all 64 banks once). Wave wv's instruction q fills
+// rows 32 wv + 8 q .. + 7, lane l the slot l % 8 of row l / 8.
+__device__ __forceinline__ uint32_t ns_sw(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4)); }
+__device__ __forceinline__ void ns_stage(const uint16_t* P, int64_t ld, int k0, int wv, int lane, uint32_t buf)
+{
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int row = 32 * wv + 8 * q + (lane >> 3);
+        load_lds16(P + row * ld + k0 + 8 * ((lane & 7) ^ ((row >> 1) & 7)), buf + (uint32_t)((4 * wv + q) * 1024));
+    }
+}
+// ... and of one whose rows are the depth: 64 rows of 128, 256 bytes a row, chunks swizzled by 4 (row % 4) for the
+// transposing reads (four rows by four chunks at a time).
+__device__ __forceinline__ uint32_t ns_tsw(int row, int chunk) { return (uint32_t)(row * 256 + ((chunk ^ (4 * (row & 3))) << 4)); }
+__device__ __forceinline__ void ns_stage_t(const uint16_t* P, int64_t ld, int k0, int wv, int lane, uint32_t buf)
+{
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int row = 16 * wv + 4 * q + (lane >> 4);
+        load_lds16(P + (int64_t)(k0 + row) * ld + 8 * ((lane & 15) ^ (4 * (row & 3))),
+                   buf + (uint32_t)((4 * wv + q) * 1024));
+    }
+}
+
+enum NSMode { NS_GRAM, NS_POLY, NS_UPDATE, NS_LAST };
+
+struct NSArgs {
+    const uint16_t *p, *q;  // operands: p [..][K] rows of the output; q [..][K] columns (gram, poly) or [K][..] (update)
+    int64_t ldp, ldq, sp, sq;
+    int K, tiles_m, tiles_n, np, mp;
+    uint16_t *out, *out_lo;  // A, B or the next X's hi; lo (read and written in place)
+    const uint16_t* in_hi;   // poly: A; update: X's hi
+    float a, b, c;
+    uint16_t* bf;  // last: the caller's matrix
+    int64_t ldb, sb;
+    int m, n, tall;
+};
+
+// C = P Q^T (gram, poly: lower tiles, each stored twice) or P Q (update): 128 x 128 tiles, four waves of 64 x 64, two
+// LDS stages filled by direct loads.
+template <int MODE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void ns_product_kernel(NSArgs g)
+{
+    constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
+    __shared__ __align__(16) uint8_t lds[2][2][NS_OPB];
+    const int lane = (int)(threadIdx.x & 63), wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int li = lane & 31, half = lane >> 5, grp = lane >> 4, i16 = lane & 15;
+    const int64_t batch = blockIdx.y;
+    const int id = (int)xcd_remap(blockIdx.x, gridDim.x);
+    int I, J;
+    if (SYM) {  // tile `id` of the lower triangle, row by row
+        I = (int)((sqrtf(8.0f * (float)id + 1.0f) - 1.0f) * 0.5f);
+        while (I * (I + 1) / 2 > id) --I;
+        while ((I + 1) * (I + 2) / 2 <= id) ++I;
+        J = id - I * (I + 1) / 2;
+    } else {
+        I = id % g.tiles_m;
+        J = id / g.tiles_m;
+    }
+    const uint16_t* P = g.p + batch * g.sp + (int64_t)I * NS_T * g.ldp;
+    const uint16_t* Q = g.q + batch * g.sq + (SYM ? (int64_t)J * NS_T * g.ldq : (int64_t)J * NS_T);
+    const uint32_t base = lds_addr(lds);
+    auto stage = [&](int st) {
+        const uint32_t buf = base + (uint32_t)((st & 1) * 2 * NS_OPB);
+        ns_stage(P, g.ldp, st * NS_K, wv, lane, buf);
+        if (SYM)
+            ns_stage(Q, g.ldq, st * NS_K, wv, lane, buf + NS_OPB);
+        else
+            ns_stage_t(Q, g.ldq, st * NS_K, wv, lane, buf + NS_OPB);
+    };
+    const int wm = 64 * (wv >> 1), wn = 64 * (wv & 1);
+    lamq_ns_f32x16 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+    const int nst = g.K / NS_K;
+    stage(0);
+    for (int st = 0; st < nst; ++st) {
+        wait_vm<0>();     // this wave's loads of the stage have landed
+        __syncthreads();  // everyone's; the other buffer is free
+        if (st + 1 < nst) stage(st + 1);
+        const uint8_t* pl = lds[st & 1][0];
+        const uint8_t* ql = lds[st & 1][1];
+        const uint32_t qb = base + (uint32_t)(((st & 1) * 2 + 1) * NS_OPB);
+#pragma unroll
+        for (int ks = 0; ks < NS_K / 16; ++ks) {
+            lamq_ns_f16x8 pf[2], qf[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                pf[i] = *reinterpret_cast<const lamq_ns_f16x8*>(pl + ns_sw(wm + 32 * i + li, 2 * ks + half));
+                if (SYM) {
+                    qf[i] = *reinterpret_cast<const lamq_ns_f16x8*>(ql + ns_sw(wn + 32 * i + li, 2 * ks + half));
+                } else {
+                    // depth 16 ks + 8 half + {0..7} of column wn + 32 i + li: two transposing reads of four each
+                    const int row = 16 * ks + 8 * half + (i16 >> 2), col = wn + 32 * i + 16 * (grp & 1) + 4 * (i16 & 3);
+                    const uint32_t a0 = qb + ns_tsw(row, col >> 3) + 8 * ((col >> 2) & 1);
+                    const uint32_t a1 = qb + ns_tsw(row + 4, col >> 3) + 8 * ((col >> 2) & 1);
+                    const lamq_ns_s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)a0);
+                    const lamq_ns_s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)a1);
+                    const short __attribute__((ext_vector_type(8))) x =
+                        __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
+                    qf[i] = __builtin_bit_cast(lamq_ns_f16x8, x);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    // gram and poly: the operands exchanged, so that a lane's four registers in a row are neighbours of
+                    // a row of the (symmetric) result; update: lane li holds row li of P's
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf[j], pf[i], acc[i][j], 0, 0, 0);
+        }
+    }
+    // result: lane's row of C wm + 32 i + li, columns wn + 32 j + 8 r + 4 half + {0..3} in registers 4 r .. 4 r + 3
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = I * NS_T + wm + 32 * i + li;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int col = J * NS_T + wn + 32 * j + 8 * r + 4 * half;
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * r + e] * NS_UNSCALE;
+                if (SYM) {
+                    const int64_t at = batch * g.mp * g.mp + (int64_t)row * g.mp + col;
+                    lamq_ns_f16x4 o;
+                    if (MODE == NS_POLY) {
+                        const lamq_ns_f16x4 A = *reinterpret_cast<const lamq_ns_f16x4*>(g.in_hi + at);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = fmaf(g.b, (float)A[e], g.c * x[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = (_Float16)x[e];
+                    *reinterpret_cast<lamq_ns_f16x4*>(g.out + at) = o;
+                    if (I != J) {
+                        uint16_t* t = g.out + batch * g.mp * g.mp + (int64_t)col * g.mp + row;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const _Float16 y = o[e];  // a bit cast of the element itself would read the first one's bits
+                            t[(int64_t)e * g.mp] = __builtin_bit_cast(uint16_t, y);
+                        }
+                    }
+                } else {
+                    const int64_t at = batch * g.mp * g.np + (int64_t)row * g.np + col;
+                    const lamq_ns_f16x4 H = *reinterpret_cast<const lamq_ns_f16x4*>(g.in_hi + at);
+                    const lamq_ns_f16x4 L = *reinterpret_cast<const lamq_ns_f16x4*>(g.out_lo + at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = fmaf(g.a, (float)H[e] + (float)L[e], x[e]);
+                    if (MODE == NS_UPDATE) {
+                        lamq_ns_f16x4 h, l;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            h[e] = (_Float16)x[e];
+                            l[e] = (_Float16)(x[e] - (float)h[e]);
+                        }
+                        *reinterpret_cast<lamq_ns_f16x4*>(g.out + at) = h;
+                        *reinterpret_cast<lamq_ns_f16x4*>(g.out_lo + at) = l;
+                    } else if (row < g.m) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (col + e < g.n) {
+                                const int64_t to = g.tall ? (int64_t)(col + e) * g.ldb + row : (int64_t)row * g.ldb + col + e;
+                                g.bf[batch * g.sb + to] = __builtin_bit_cast(uint16_t, (__bf16)(x[e] * NS_UNSCALE));
+                            }
+                    }
+                }
+            }
+    }
+}
+
+// G as bf16: the result of no step at all
+template <typename Elt>
+__global__ __launch_bounds__(256) void ns_copy_kernel(const Elt* __restrict__ G, int64_t rows, int64_t cols, int64_t ld,
+                                                      int64_t stride, const double* __restrict__ parts, int nparts,
+                                                      uint16_t* __restrict__ out, int64_t ldo, int64_t so)
+{
+    const double ss = ns_sum((int)threadIdx.x < nparts ? parts[blockIdx.y * nparts + threadIdx.x] : 0.0);
+    const double f = ss > 0.0 ? 1.0 / sqrt(ss) : ss;
+    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < rows * cols; i += 256 * (int64_t)gridDim.x) {
+        const int64_t r = i / cols, c = i % cols;
+        const float v = (float)((double)ns_load(G + blockIdx.y * stride + r * ld + c) * f);
+        out[blockIdx.y * so + r * ldo + c] = __builtin_bit_cast(uint16_t, (__bf16)v);
+    }
+}
+
+struct NSPlan {
+    int64_t m, n, mp, np;
+    size_t x, aa, total;  // bytes of one [mp][np] and [mp][mp] array over the batch, and of everything
+};
+static NSPlan ns_plan(int64_t batch, int64_t rows, int64_t cols)
+{
+    NSPlan p;
+    p.m = rows < cols ? rows : cols;
+    p.n = rows < cols ? cols : rows;
+    p.mp = cdiv(p.m, NS_T) * NS_T;
+    p.np = cdiv(p.n, NS_T) * NS_T;
+    p.x = (size_t)batch * p.mp * p.np * 2;
+    p.aa = (size_t)batch * p.mp * p.mp * 2;
+    p.total = (size_t)batch * NS_PARTS * sizeof(double) + 3 * p.x + 2 * p.aa;
+    return p;
+}
+
+extern "C" size_t lamq_orthogonalize_workspace_size(int64_t batch, int64_t rows, int64_t cols)
+{
+    if (batch < 1 || rows < 1 || cols < 1) return 0;
+    return ns_plan(batch, rows, cols).total;
+}
+
+// The largest singular value that any step reaches from [0, 1], on a grid of them: what the float16 range is checked
+// against.
+static double ns_reach(int steps, double a, double b, double c)
+{
+    double s[256], top = 1.0;
+    for (int i = 0; i < 256; ++i) s[i] = (i + 1) / 256.0;
+    for (int k = 0; k < steps && top < 1e6; ++k)
+        for (int i = 0; i < 256; ++i) {
+            s[i] = s[i] * (a + s[i] * s[i] * (b + s[i] * s[i] * c));
+            top = fabs(s[i]) <= top ? top : fabs(s[i]) < 1e6 ? fabs(s[i]) : 1e6;  // a NaN counts as past it
+        }
+    return top;
+}
+
+template <typename Elt>
+static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, int64_t ld, int64_t stride, int steps, float a,
+                     float b, float c, uint16_t* out, int64_t ldo, int64_t so, void* workspace, size_t workspace_bytes,
+                     void* stream)
+{
+    if (!G || !out || batch < 0 || rows < 0 || cols < 0 || steps < 0 || ld < cols || ldo < cols) return LAMQ_EINVAL;
+    if (batch > 1 && (stride < 0 || so < rows * ldo)) return LAMQ_EINVAL;
+    if ((uintptr_t)G % sizeof(Elt) || (uintptr_t)out % 2) return LAMQ_EINVAL;
+    if (!(ns_reach(steps, a, b, c) <= 8.0)) return LAMQ_EINVAL;
+    if (batch == 0 || rows == 0 || cols == 0) return LAMQ_OK;
+    if (batch > 65535 || rows > (1 << 20) || cols > (1 << 20)) return LAMQ_EUNSUP;
+    const NSPlan p = ns_plan(batch, rows, cols);
+    if (p.mp * p.np > ((int64_t)1 << 36)) return LAMQ_EUNSUP;
+    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < p.total) return LAMQ_EINVAL;
+    hipStream_t st = as_stream(stream);
+    double* parts = reinterpret_cast<double*>(workspace);
+    uint8_t* at = reinterpret_cast<uint8_t*>(parts + batch * NS_PARTS);
+    uint16_t* hi[2] = {reinterpret_cast<uint16_t*>(at), reinterpret_cast<uint16_t*>(at + p.x)};
+    uint16_t* lo = reinterpret_cast<uint16_t*>(at + 2 * p.x);
+    uint16_t* A = reinterpret_cast<uint16_t*>(at + 3 * p.x);
+    uint16_t* Bm = reinterpret_cast<uint16_t*>(at + 3 * p.x + p.aa);
+    const int64_t want = cdiv(rows * cols, 4096);
+    const int nparts = (int)(want < NS_PARTS ? want : NS_PARTS);
+    hipLaunchKernelGGL(ns_norm_kernel<Elt>, dim3(nparts, (unsigned)batch), dim3(256), 0, st, G, rows, cols, ld, stride, parts);
+    LAMQ_LAUNCH_CHECK();
+    const bool tall = rows > cols;
+    if (steps == 0) {
+        hipLaunchKernelGGL(ns_copy_kernel<Elt>, dim3(nparts, (unsigned)batch), dim3(256), 0, st, G, rows, cols, ld, stride,
+                           parts, nparts, out, ldo, so);
+        LAMQ_LAUNCH_CHECK();
+        return LAMQ_OK;
+    }
+    const dim3 sg((unsigned)(p.np / 64), (unsigned)(p.mp / 64), (unsigned)batch);
+    if (tall)
+        hipLaunchKernelGGL((ns_start_kernel<Elt, true>), sg, dim3(256), 0, st, G, rows, cols, ld, stride, parts, nparts,
+                           (int)p.mp, (int)p.np, hi[0], lo);
+    else
+        hipLaunchKernelGGL((ns_start_kernel<Elt, false>), sg, dim3(256), 0, st, G, rows, cols, ld, stride, parts, nparts,
+                           (int)p.mp, (int)p.np, hi[0], lo);
+    LAMQ_LAUNCH_CHECK();
+    const int tm = (int)(p.mp / NS_T), tn = (int)(p.np / NS_T);
+    NSArgs x{};
+    x.np = (int)p.np;
+    x.mp = (int)p.mp;
+    x.tiles_m = tm;
+    x.tiles_n = tn;
+    x.a = a;
+    x.b = b;
+    x.c = c;
+    x.out_lo = lo;
+    x.bf = out;
+    x.ldb = ldo;
+    x.sb = so;
+    x.m = (int)p.m;
+    x.n = (int)p.n;
+    x.tall = tall;
+    const dim3 lower((unsigned)(tm * (tm + 1) / 2), (unsigned)batch), full((unsigned)(tm * tn), (unsigned)batch);
+    for (int k = 0; k < steps; ++k) {
+        NSArgs y = x;
+        y.p = y.q = hi[k & 1];
+        y.ldp = y.ldq = p.np;
+        y.sp = y.sq = p.mp * p.np;
+        y.K = (int)p.np;
+        y.out = A;
+        hipLaunchKernelGGL(ns_product_kernel<NS_GRAM>, lower, dim3(256), 0, st, y);
+        LAMQ_LAUNCH_CHECK();
+        y.p = y.q = y.in_hi = A;
+        y.ldp = y.ldq = p.mp;
+        y.sp = y.sq = p.mp * p.mp;
+        y.K = (int)p.mp;
+        y.out = Bm;
+        hipLaunchKernelGGL(ns_product_kernel<NS_POLY>, lower, dim3(256), 0, st, y);
+        LAMQ_LAUNCH_CHECK();
+        y.p = Bm;
+        y.q = y.in_hi = hi[k & 1];
+        y.ldq = p.np;
+        y.sq = p.mp * p.np;
+        y.out = hi[1 - (k & 1)];
+        if (k + 1 < steps)
+            hipLaunchKernelGGL(ns_product_kernel<NS_UPDATE>, full, dim3(256), 0, st, y);
+        else
+            hipLaunchKernelGGL(ns_product_kernel<NS_LAST>, full, dim3(256), 0, st, y);
+        LAMQ_LAUNCH_CHECK();
+    }
+    return LAMQ_OK;
+}
+
+extern "C" int lamq_orthogonalize_bf16(const uint16_t* G, int64_t batch, int64_t rows, int64_t cols, int64_t ld,
+                                       int64_t stride, int steps, float a, float b, float c, uint16_t* out, int64_t ldo,
+                                       int64_t so, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return ns_launch(G, batch, rows, cols, ld, stride, steps, a, b, c, out, ldo, so, workspace, workspace_bytes, stream);
+}
+
+extern "C" int lamq_orthogonalize_f32(const float* G, int64_t batch, int64_t rows, int64_t cols, int64_t ld,
+                                      int64_t stride, int steps, float a, float b, float c, uint16_t* out, int64_t ldo,
+                                      int64_t so, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return ns_launch(G, batch, rows, cols, ld, stride, steps, a, b, c, out, ldo, so, workspace, workspace_bytes, stream);
+}

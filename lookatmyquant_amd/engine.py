@@ -717,6 +717,40 @@ def attention_causal_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, 
     return dq, dk, dv
 
 
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # a quintic that takes singular values from 0.002 to near 1 in five steps
+
+
+def orthogonalize(G: torch.Tensor, steps: int = 5, coeffs: tuple = NEWTON_SCHULZ,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """The Newton-Schulz orthogonalisation of an update (lamq_orthogonalize_bf16, _f32): G [m, n] or a batch [b, m, n],
+    bf16 or float32, each matrix scaled by its Frobenius norm and taken `steps` times through a X + (b A + c A^2) X, A =
+    X X^T on the short side, (a, b, c) = coeffs. Returns bf16 of G's shape, into `out` if given. Coefficients whose
+    polynomial carries a singular value in [0, 1] past 8 are refused."""
+    dt = G.dtype if G.dtype in (torch.bfloat16, torch.float32) else torch.bfloat16
+    need(G, dt, "G")
+    if G.dim() not in (2, 3):
+        raise ValueError("G must be a matrix or a batch of matrices")
+    if len(coeffs) != 3 or steps < 0:
+        raise ValueError("three coefficients and a number of steps")
+    if out is None:
+        out = torch.empty(G.shape, dtype=torch.bfloat16, device=G.device)
+    need(out, torch.bfloat16, "out")
+    if out.shape != G.shape or out.device != G.device:
+        raise ValueError("out must have G's shape and device")
+    batch, (m, n) = (G.shape[0] if G.dim() == 3 else 1), G.shape[-2:]
+    if G.numel() == 0:
+        return out
+    # the stride of an axis of one entry is not used and may be anything
+    row = lambda t: t.stride(-2) if m > 1 else n
+    step = lambda t: t.stride(0) if batch > 1 else m * row(t)
+    nbytes = lib().lamq_orthogonalize_workspace_size(batch, m, n)
+    ws = workspace(nbytes, G.device)
+    fn = lib().lamq_orthogonalize_bf16 if dt == torch.bfloat16 else lib().lamq_orthogonalize_f32
+    check(fn(ptr(G), batch, m, n, row(G), step(G), int(steps), *(float(x) for x in coeffs), ptr(out), row(out), step(out),
+             ptr(ws), nbytes, stream(G.device)), "orthogonalize")
+    return out
+
+
 class EventLog(dict):
     """key -> list of (start, end) torch.cuda.Event pairs. lead_cycles > 0: before each span's start event, a GPU spin
     of that many cycles (torch.cuda._sleep) keeps the stream busy while the host enqueues the span, so that a span

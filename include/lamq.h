@@ -482,7 +482,8 @@ int lamq_attention_causal_bf16(const uint16_t* q, int64_t sqb, int64_t sqh, int6
  *   lens  [B] int32 on the device, or NULL (all T): tokens past lens[b] (held to 0 .. T) are padding. Nothing is
  *         read there; their rows of out and of the gradients are zeros, their lse -inf.
  * Sums, scores and dP are float32; P and dS are rounded to bf16 as operands of the next product, each result once.
- * The results do not depend on scheduling. Limits as lamq_attention_causal_bf16.
+ * The results do not depend on scheduling. Limits as lamq_attention_causal_bf16; the backward's token strides at most
+ * 16,777,215 (LAMQ_EUNSUP above).
  * ---------------------------------------------------------------------------------------------- */
 typedef struct {
     uint16_t* data;

@@ -49,3 +49,14 @@ struct AtOut {
     uint16_t* p;
     int64_t sb, sh, st;
 };
+
+// One direct global->LDS load (16 bytes a lane into m0 + 16 * lane) from a uniform address and a 32-bit byte offset a
+// lane; M0 saved and restored around it, with the wait state its write needs (load_lds16).
+__device__ __forceinline__ void at_load_lds16(const uint16_t* base, uint32_t off, uint32_t m)
+{
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(off), "s"(base), "s"(m)
+                 : "memory");
+}

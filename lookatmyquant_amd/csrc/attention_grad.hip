@@ -6,7 +6,7 @@
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,  dK and dV summed over a key/value head's query heads.
 //
 // Two kernels, so that each gradient has one owner and its sums one order (no atomics): attention_dq_kernel owns 128
-// queries and walks the keys up to them, forming S^T, dP^T and dQ^T += K^T dS^T; attention_dkdv_kernel owns 128 keys and
+// queries and walks the keys up to them, forming S^T, dP^T and dQ^T += K^T dS^T; attention_dkdv_kernel owns 64 keys and
 // walks the query heads and queries from them on, forming S, dP, dV^T += dO^T P and dK^T += Q^T dS. Seven products where
 // five would do with one pass; the two formed twice cost less than a float32 dQ added up in memory (a read and a
 // write of 4 bytes per query, head dim and key block) and keep the results the same from run to run.
@@ -23,8 +23,10 @@
 
 #define AG_R 32                       // rows a wave owns
 #define AG_W 64                       // rows of a walked block
-#define AG_OWN 128                    // rows a workgroup owns
+#define AG_OWN 128                    // queries a workgroup owns
+#define AG_KEYS 64                    // keys a workgroup owns
 #define AG_OPB (AG_W * AT_D * 2)      // bytes of one operand's block (16 KB)
+#define AG_HALF (AG_OPB / 2)          // ... and of 32 of its rows
 
 __device__ __forceinline__ int at_f(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
 __device__ __forceinline__ uint32_t at_fsw(int row, int chunk)
@@ -32,33 +34,48 @@ __device__ __forceinline__ uint32_t at_fsw(int row, int chunk)
     return (uint32_t)(row * (AT_D * 2) + ((chunk ^ at_f(row)) << 4));
 }
 
-// A block of 64 rows r0 .. of an operand into LDS (global_load_lds, 16 bytes a lane): wave wv's instruction q fills rows
-// 16 wv + 4 q .. + 3, lane l the slot l % 16 of row 16 wv + 4 q + l / 16. Rows past `last` read row `last`.
-__device__ __forceinline__ void ag_load_block(const uint16_t* __restrict__ base, int64_t st, int r0, int last, int wv,
-                                              int lane, uint32_t buf)
+// A block of walked rows into LDS (at_load_lds16): wave wv's instruction q fills rows 16 wv + 4 q .. + 3, lane l the
+// slot l % 16 of row 16 wv + 4 q + l / 16 with the chunk that belongs there. Of fewer than 64 rows the ones past the
+// last read the last one (and meet probabilities of 0).
+__device__ __forceinline__ void ag_load_block(const uint16_t* block, int64_t st, int rows, int wv, int lane, uint32_t buf)
 {
+    const int sub = lane >> 4;
+    uint32_t chunk = 16u * (uint32_t)((lane & 15) ^ (sub << 2));  // of q = 0; q's is chunk ^ 16 q
+    uint32_t off = (uint32_t)sub * (uint32_t)(2 * st);
+    asm volatile("" : "+v"(chunk), "+v"(off));  // formed here, not kept in eight registers around the loop
+    if (rows >= AG_W) {
+        const uint16_t* p = block + 16 * wv * st;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int row = r0 + 16 * wv + 4 * q + (lane >> 4);
-        const int chunk = (lane & 15) ^ (((lane >> 4) << 2) | q);
-        load_lds16(base + (int64_t)(row < last ? row : last) * st + 8 * chunk, buf + (uint32_t)((4 * wv + q) * 1024));
+        for (int q = 0; q < 4; ++q)
+            at_load_lds16(p + 4 * q * st, off + (chunk ^ (16u * q)), buf + (uint32_t)((4 * wv + q) * 1024));
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = 16 * wv + 4 * q + sub;
+            at_load_lds16(block, (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)(2 * st) + (chunk ^ (16u * q)),
+                          buf + (uint32_t)((4 * wv + q) * 1024));
+        }
     }
 }
 
-// A operand of a product over the head dim: rows 32 hf + li, head dims 16 j + 8 hi .. + 7
-__device__ __forceinline__ lamq_at_bf16x8 ag_frag(const uint8_t* buf, int row, int j, int hi)
+// LDS addresses of a lane's operand fragments in a block (64 rows of 256 bytes, aligned to 256), from two bases:
+// A operand of a product over the head dim: row `row` (32 hf + li), head dims 16 j + 8 hi .. + 7, chunk 2 j + hi.
+__device__ __forceinline__ uint32_t ag_frag_base(int row, int hi) { return at_fsw(row, hi); }
+__device__ __forceinline__ lamq_at_bf16x8 ag_frag(uint32_t base, int j, uint32_t block)
 {
-    return *reinterpret_cast<const lamq_at_bf16x8*>(buf + at_fsw(row, 2 * j + hi));
+    typedef __attribute__((address_space(3))) const lamq_at_bf16x8 lds_frag;
+    return *(lds_frag*)(uintptr_t)((base ^ (32u * j)) + block);
 }
-
-// A operand of a product over the walked rows: head dims 32 t + li, rows 32 hf + 16 mi + 4 hi + {0..3} and + 8
-__device__ __forceinline__ lamq_at_bf16x8 ag_tr_frag(uint32_t buf, int hf, int mi, int t, int lane)
+// A operand of a product over the walked rows: head dims 32 t + li, rows 32 hf + 16 mi + 4 hi + {0..3} and + 8 (the row
+// eight further on differs by 2 in at_f, the one sixteen further on not at all).
+__device__ __forceinline__ uint32_t ag_tr_base(int hf, int lane)
 {
-    const int hi = lane >> 5, g = lane >> 4, i16 = lane & 15;
-    const int row = 32 * hf + 16 * mi + 4 * hi + (i16 >> 2);
-    const int col = 32 * t + 16 * (g & 1) + 4 * (i16 & 3);
-    const uint32_t a0 = buf + at_fsw(row, col >> 3) + 8 * ((col >> 2) & 1);
-    const uint32_t a1 = buf + at_fsw(row + 8, col >> 3) + 8 * ((col >> 2) & 1);
+    const int i16 = lane & 15, col = 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+    return at_fsw(32 * hf + 4 * (lane >> 5) + (i16 >> 2), col >> 3) + 8 * ((col >> 2) & 1);
+}
+__device__ __forceinline__ lamq_at_bf16x8 ag_tr_frag(uint32_t base, int mi, int t, uint32_t block)
+{
+    const uint32_t a0 = (base ^ (64u * t)) + block + 4096u * mi, a1 = (base ^ (64u * t) ^ 32u) + block + 4096u * mi + 2048u;
     const lamq_at_s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_at_lds_s4*)(uintptr_t)a0);
     const lamq_at_s4 up = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_at_lds_s4*)(uintptr_t)a1);
     const short __attribute__((ext_vector_type(8))) w = __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -120,7 +137,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int32_t* __restrict__ lens, float* __restrict__ stats, int64_t nstats, int rep, int Hkv, int pairs, int Tall,
     float scale, float scale_log2)
 {
-    __shared__ __align__(16) uint8_t lds[2][2][AG_OPB];  // [buffer][K, V]
+    __shared__ __align__(256) uint8_t lds[2][2][AG_OPB];  // [buffer][K, V]
     const int nqb = (Tall + AG_OWN - 1) / AG_OWN;
     int pair, rem;
     if (!ag_place(pairs, nqb * rep, pair, rem)) return;
@@ -144,8 +161,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int my_last = q0 < T ? (q0 + AG_R < T ? q0 + AG_R : T) - 1 : -1;
     auto load_block = [&](int kb) {
         const uint32_t buf = base + (uint32_t)((kb & 1) * 2 * AG_OPB);
-        ag_load_block(Kp, K.st, kb * AG_W, T - 1, wv, lane, buf);
-        ag_load_block(Vp, V.st, kb * AG_W, T - 1, wv, lane, buf + AG_OPB);
+        const int r0 = kb * AG_W;
+        ag_load_block(Kp + r0 * K.st, K.st, T - r0, wv, lane, buf);
+        ag_load_block(Vp + r0 * V.st, V.st, T - r0, wv, lane, buf + AG_OPB);
     };
     load_block(0);
     lamq_at_bf16x8 qf[8], df[8];
@@ -185,9 +203,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         __syncthreads();  // everyone's; the other buffer is free
         if (kb + 1 < nblk) load_block(kb + 1);
         const int k0 = kb * AG_W;
-        const uint8_t* kl = lds[kb & 1][0];
-        const uint8_t* vl = lds[kb & 1][1];
-        const uint32_t kbase = base + (uint32_t)((kb & 1) * 2 * AG_OPB);
+        uint32_t fb = base + (uint32_t)((kb & 1) * 2 * AG_OPB) + ag_frag_base(li, hi);
+        uint32_t tb = base + (uint32_t)((kb & 1) * 2 * AG_OPB) + ag_tr_base(0, lane);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
             if (k0 + 32 * hf > my_last) continue;  // uniform: past this wave's queries
@@ -199,8 +216,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(kl, 32 * hf + li, j, hi), qf[j], s, 0, 0, 0);
-                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(vl, 32 * hf + li, j, hi), df[j], dp, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(fb, j, hf * AG_HALF), qf[j], s, 0, 0, 0);
+                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(fb, j, AG_OPB + hf * AG_HALF), df[j], dp, 0, 0, 0);
             }
             if (k0 + 32 * hf + 31 > q0) {  // the causal mask, only where the half reaches past the wave's first query
 #pragma unroll
@@ -215,51 +232,60 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
-                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(kbase, hf, mi, t, lane), dsf[mi], acc[t],
+                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(tb, mi, t, hf * AG_HALF), dsf[mi], acc[t],
                                                                      0, 0, 0);
         }
     }
     if (myq < T) ag_store_row(dQp + (int64_t)myq * dQ.st, acc, scale, hi);
 }
 
-// dK and dV of 128 keys of a key/value head, over its query heads and the queries from the keys on.
+// dK and dV of 64 keys of a key/value head, over its query heads and the queries from the keys on. Two waves own 32 keys
+// each, two more the same keys: of a walked block of 64 queries the first pair takes the first 32, the second the
+// others, and their sums are joined in LDS at the end. A wave's walk is as long as the heads and the queries are many,
+// so with 128 keys a workgroup four sequences of 2,048 had 512 workgroups, one for every slot of the chip, the first
+// keys' with twice the mean walk: 606 us; halved walks of half the keys go out longest first and fill each other's
+// tails. The queries are walked from the last one down, so that workgroups that start together read the same blocks.
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_dkdv_kernel(
     AtView Q, AtView K, AtView V, AtView dO, AtOut dK, AtOut dV, const int32_t* __restrict__ lens,
     const float* __restrict__ stats, int64_t nstats, int rep, int Hkv, int pairs, int Tall, float scale, float scale_log2)
 {
-    __shared__ __align__(16) uint8_t lds[2][2][AG_OPB];  // [buffer][Q, dO]
+    __shared__ __align__(256) uint8_t lds[2][2][AG_OPB];  // [buffer][Q, dO]; at the end [wave][64 registers][64 lanes]
     __shared__ __align__(16) float row_stats[2][2][AG_W];  // [buffer][lse, delta]
-    const int nkb = (Tall + AG_OWN - 1) / AG_OWN;
-    int pair, kb;
-    if (!ag_place(pairs, nkb, pair, kb)) return;  // the first keys have the most queries: they go out first
+    const int nkb = (Tall + AG_KEYS - 1) / AG_KEYS;
+    // workgroup -> (key block, pair): the first keys, whose walks are the longest, go out first
+    const int id = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+    if ((unsigned)id >= (unsigned)pairs * (unsigned)nkb) return;
+    const int pair = id % pairs, kb = id / pairs;
     const int b = pair / Hkv, hk = pair % Hkv;
     const int lane = (int)(threadIdx.x & 63), wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int li = lane & 31, hi = lane >> 5;
+    const int li = lane & 31, hi = lane >> 5, kw = wv >> 1, qw = wv & 1;
     const int T = at_length(lens, b, Tall);
     uint16_t* dKp = dK.p + b * dK.sb + (int64_t)hk * dK.sh;
     uint16_t* dVp = dV.p + b * dV.sb + (int64_t)hk * dV.sh;
-    const int own0 = kb * AG_OWN, own1 = own0 + AG_OWN < Tall ? own0 + AG_OWN : Tall;
+    const int own0 = kb * AG_KEYS, own1 = own0 + AG_KEYS < Tall ? own0 + AG_KEYS : Tall;
     if (own1 > T) {
         const int first = own0 > T ? own0 : T;
         at_zero_rows(dKp, dK.st, first, own1);
         at_zero_rows(dVp, dV.st, first, own1);
         if (own0 >= T) return;  // uniform, before any barrier
     }
-    const int k0 = own0 + AG_R * wv, myk = k0 + li, krow = myk < T ? myk : T - 1;
+    const int k0 = own0 + AG_R * kw, myk = k0 + li, krow = myk < T ? myk : T - 1;
     const uint32_t base = lds_addr(lds), sbase = lds_addr(row_stats);
-    const int b0 = own0 / AG_W, nblk = (T - 1) / AG_W - b0 + 1, items = rep * nblk;
-    auto load_block = [&](int it) {
-        const int h = hk * rep + it / nblk, r0 = (b0 + it % nblk) * AG_W;
-        const uint32_t buf = base + (uint32_t)((it & 1) * 2 * AG_OPB);
-        ag_load_block(Q.p + b * Q.sb + (int64_t)h * Q.sh, Q.st, r0, T - 1, wv, lane, buf);
-        ag_load_block(dO.p + b * dO.sb + (int64_t)h * dO.sh, dO.st, r0, T - 1, wv, lane, buf + AG_OPB);
+    const int b0 = own0 / AG_W, b1 = (T - 1) / AG_W;  // the walked blocks, from b1 down to b0
+    auto load_block = [&](int h, int blk, int to) {
+        const int r0 = blk * AG_W;
+        const uint32_t buf = base + (uint32_t)(to * 2 * AG_OPB);
+        ag_load_block(Q.p + b * Q.sb + (int64_t)h * Q.sh + r0 * Q.st, Q.st, T - r0, wv, lane, buf);
+        ag_load_block(dO.p + b * dO.sb + (int64_t)h * dO.sh + r0 * dO.st, dO.st, T - r0, wv, lane, buf + AG_OPB);
         if (wv < 2) {
             const int row = r0 + lane < T ? r0 + lane : T - 1;
             load_lds4(stats + wv * nstats + ((int64_t)b * Hkv * rep + h) * Tall + row,
-                      sbase + (uint32_t)(((it & 1) * 2 + wv) * AG_W * 4));
+                      sbase + (uint32_t)((to * 2 + wv) * AG_W * 4));
         }
     };
-    load_block(0);
+    const int h1 = hk * rep + rep;
+    int h = hk * rep, blk = b1;
+    load_block(h, blk, 0);
     lamq_at_bf16x8 kf[8], vf[8];
     {
         const uint16_t* Kr = K.p + b * K.sb + (int64_t)hk * K.sh + (int64_t)krow * K.st + 8 * hi;
@@ -277,69 +303,86 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int v = 0; v < 16; ++v) dk[t][v] = dv[t][v] = 0.0f;
-    for (int it = 0; it < items; ++it) {
+    for (int cur = 0; h < h1; cur ^= 1) {
         wait_vm<0>();     // this wave's loads of the block have landed
         __syncthreads();  // everyone's; the other buffer is free
-        if (it + 1 < items) load_block(it + 1);
-        const int r0 = (b0 + it % nblk) * AG_W;
-        const uint8_t* ql = lds[it & 1][0];
-        const uint8_t* dl = lds[it & 1][1];
-        const uint32_t qbase = base + (uint32_t)((it & 1) * 2 * AG_OPB), dbase = qbase + AG_OPB;
-#pragma unroll 1
-        for (int hf = 0; hf < 2; ++hf) {
-            const int q0 = r0 + 32 * hf;
-            if (q0 + 31 < k0 || q0 >= T) continue;  // uniform: no query here sees this wave's keys
-            const float* sl = &row_stats[it & 1][0][32 * hf + 4 * hi];
-            lamq_at_f32x16 s, dp;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float4 dl4 = *reinterpret_cast<const float4*>(sl + AG_W + 8 * r);
-                dp[4 * r] = -dl4.x;
-                dp[4 * r + 1] = -dl4.y;
-                dp[4 * r + 2] = -dl4.z;
-                dp[4 * r + 3] = -dl4.w;
-            }
-#pragma unroll
-            for (int v = 0; v < 16; ++v) s[v] = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(ql, 32 * hf + li, j, hi), kf[j], s, 0, 0, 0);
-                dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(dl, 32 * hf + li, j, hi), vf[j], dp, 0, 0, 0);
-            }
-            if (q0 < k0 + 31 || q0 + 31 >= T) {  // the causal mask and the queries past the length
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int q = q0 + 8 * (v >> 2) + 4 * hi + (v & 3);
-                    s[v] = myk <= q && q < T ? s[v] : -__builtin_inff();
-                }
-            }
-            lamq_at_bf16x8 pf[2], dsf[2];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float4 ls4 = *reinterpret_cast<const float4*>(sl + 8 * r);
-                const float ls[4] = {ls4.x, ls4.y, ls4.z, ls4.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int v = 4 * r + e;
-                    const float p = __builtin_amdgcn_exp2f(fmaf(s[v], scale_log2, -ls[e]));
-                    pf[v >> 3][v & 7] = (__bf16)p;
-                    dsf[v >> 3][v & 7] = (__bf16)(p * dp[v]);
-                }
-            }
-#pragma unroll
-            for (int mi = 0; mi < 2; ++mi)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    dv[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(dbase, hf, mi, t, lane), pf[mi], dv[t], 0, 0,
-                                                                    0);
-                    dk[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(qbase, hf, mi, t, lane), dsf[mi], dk[t], 0,
-                                                                    0, 0);
-                }
+        const int q0 = blk * AG_W + 32 * qw;  // this wave's queries of the block
+        if (--blk < b0) {
+            blk = b1;
+            ++h;
         }
+        if (h < h1) load_block(h, blk, cur ^ 1);
+        if (q0 + 31 < k0 || q0 >= T) continue;  // uniform: no query here sees this wave's keys
+        uint32_t fb = base + (uint32_t)(cur * 2 * AG_OPB) + ag_frag_base(32 * qw + li, hi);
+        uint32_t tb = base + (uint32_t)(cur * 2 * AG_OPB) + ag_tr_base(qw, lane);
+        asm volatile("" : "+v"(fb), "+v"(tb));  // the fragments' addresses formed here, not kept around the loop
+        const float* sl = &row_stats[cur][0][32 * qw + 4 * hi];
+        lamq_at_f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float4 dl4 = *reinterpret_cast<const float4*>(sl + AG_W + 8 * r);
+            dp[4 * r] = -dl4.x;
+            dp[4 * r + 1] = -dl4.y;
+            dp[4 * r + 2] = -dl4.z;
+            dp[4 * r + 3] = -dl4.w;
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(fb, j, 0), kf[j], s, 0, 0, 0);
+            dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(fb, j, AG_OPB), vf[j], dp, 0, 0, 0);
+        }
+        if (q0 < k0 + 31 || q0 + 31 >= T) {  // the causal mask and the queries past the length
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int q = q0 + 8 * (v >> 2) + 4 * hi + (v & 3);
+                s[v] = myk <= q && q < T ? s[v] : -__builtin_inff();
+            }
+        }
+        lamq_at_bf16x8 pf[2], dsf[2];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float4 ls4 = *reinterpret_cast<const float4*>(sl + 8 * r);
+            const float ls[4] = {ls4.x, ls4.y, ls4.z, ls4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = 4 * r + e;
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[v], scale_log2, -ls[e]));
+                pf[v >> 3][v & 7] = (__bf16)p;
+                dsf[v >> 3][v & 7] = (__bf16)(p * dp[v]);
+            }
+        }
+#pragma unroll
+        for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                dv[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(tb, mi, t, AG_OPB), pf[mi], dv[t], 0, 0, 0);
+                dk[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(tb, mi, t, 0), dsf[mi], dk[t], 0, 0,
+                                                                0);
+            }
     }
-    if (myk < T) {
-        ag_store_row(dKp + (int64_t)myk * dK.st, dk, scale, hi);
-        ag_store_row(dVp + (int64_t)myk * dV.st, dv, 1.0f, hi);
+    // the two halves of the queries: the first pair of waves takes the other's dK and ends with it, the second dV
+    __syncthreads();  // everyone's last block is done with
+    float* mine = reinterpret_cast<float*>(lds) + wv * 64 * 64 + lane;
+    const float* other = reinterpret_cast<float*>(lds) + (wv ^ 1) * 64 * 64 + lane;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) mine[64 * (16 * t + v)] = qw ? dk[t][v] : dv[t][v];
+    __syncthreads();
+    if (qw) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) dv[t][v] = other[64 * (16 * t + v)] + dv[t][v];
+        if (myk < T) ag_store_row(dVp + (int64_t)myk * dV.st, dv, 1.0f, hi);
+    } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) dk[t][v] += other[64 * (16 * t + v)];
+        if (myk < T) ag_store_row(dKp + (int64_t)myk * dK.st, dk, scale, hi);
     }
 }
 
@@ -366,11 +409,12 @@ extern "C" int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_h
         if (!x.data || (uintptr_t)x.data % (i < 5 ? 16 : 8)) return LAMQ_EINVAL;  // 16-byte loads, 8-byte stores
         for (int64_t s : {x.sb, x.sh, x.st})
             if (s < 0 || s % 8 != 0) return LAMQ_EINVAL;
+        if (T > 1 && x.st > 0xffffff) return LAMQ_EUNSUP;  // 64 rows within a 32-bit byte offset
     }
     if (B == 0 || T == 0) return LAMQ_OK;
     if (B > 65535 || H > 65535 || T > 0x7fffff) return LAMQ_EUNSUP;
-    const int64_t qwgs = cdiv(T, AG_OWN) * H * B, kwgs = cdiv(T, AG_OWN) * Hkv * B;
-    if (qwgs > 0x7fffffff) return LAMQ_EUNSUP;
+    const int64_t qwgs = cdiv(T, AG_OWN) * H * B, kwgs = cdiv(T, AG_KEYS) * Hkv * B;
+    if (qwgs > 0x7fffffff || kwgs > 0x7fffffff) return LAMQ_EUNSUP;
     if (!workspace || (uintptr_t)workspace % 4 ||
         workspace_bytes < lamq_attention_causal_grad_workspace_size(B, H, Hkv, T))
         return LAMQ_EINVAL;

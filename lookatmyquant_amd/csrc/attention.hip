@@ -34,8 +34,13 @@
 // 16 keys a fragment read serves at once touch 16 different chunks (all 64 banks once); V's by 4 (row & 3), so the
 // 32 lanes a transposing read serves at once touch 16 different chunks of four rows. The loads place each chunk where
 // the swizzle puts it (a lane fetches the chunk that belongs in its 16-byte slot).
-#include "attention.h"
+#include "common.h"
 
+typedef __bf16 lamq_at_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float lamq_at_f32x16 __attribute__((ext_vector_type(16)));
+
+#define AT_GRID_X (1 << 22)
+#define AT_D 128                        // head dim
 #define AT_QW 32                        // queries per wave
 #define AT_KB 32                        // keys per half block (one S^T tile)
 #define AT_KB2 64                       // keys per block in LDS
@@ -52,18 +57,28 @@ __device__ __forceinline__ uint32_t at_ksw(int row, int chunk)
     return (uint32_t)(row * (AT_D * 2) + ((chunk ^ (row & 15)) << 4));
 }
 
-// LSE: training's forward, which takes the sequences' lengths (the tokens past lens[b] are padding: no operand is read
-// there, and their outputs are written as zeros) and keeps log sum_u exp(scale q . k_u) of every query, float32
-// [B, H, T], -inf past a length: what the backward recomputes the probabilities from.
-template <bool LSE>
+typedef short lamq_at_s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) lamq_at_s4 lamq_at_lds_s4;
+
+// the larger of this lane's value and lane ^ 32's (one swap of the wave's halves, no LDS)
+__device__ __forceinline__ float at_max32(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float at_sum32(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_causal_kernel(
     const uint16_t* __restrict__ Q, int64_t sqb, int64_t sqh, int64_t sqt, const uint16_t* __restrict__ K,
     int64_t skb, int64_t skh, int64_t skt, const uint16_t* __restrict__ V, int64_t svb, int64_t svh, int64_t svt,
-    uint16_t* __restrict__ O, int64_t sob, int64_t soh, int64_t sot, int rep, int Hkv, int pairs, int Tall,
-    float scale_log2, const int32_t* __restrict__ lens, float* __restrict__ lse)
+    uint16_t* __restrict__ O, int64_t sob, int64_t soh, int64_t sot, int rep, int Hkv, int pairs, int T, float scale_log2)
 {
     __shared__ __align__(16) uint8_t lds[2][2][AT_OPB];  // [buffer][K, V]
-    const int nqb = (Tall + AT_QB - 1) / AT_QB;
+    const int nqb = (T + AT_QB - 1) / AT_QB;
     // workgroup -> (pair of sequence and key/value head, query head of the pair, query block)
     int pair, rem;
     {
@@ -84,14 +99,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int wv = __builtin_amdgcn_readfirstlane(wave);
     const int q0 = qb * AT_QB + AT_QW * wv;
     const int li = lane & 31, hi = lane >> 5, g = lane >> 4, i16 = lane & 15;
-    const int T = LSE ? at_length(lens, b, Tall) : Tall;
-    if (LSE && qb * AT_QB + AT_QB > T) {  // the rows past the sequence's end
-        const int first = qb * AT_QB > T ? qb * AT_QB : T, last = qb * AT_QB + AT_QB < Tall ? qb * AT_QB + AT_QB : Tall;
-        at_zero_rows(O + b * sob + (int64_t)h * soh, sot, first, last);
-        float* L = lse + ((int64_t)b * Hkv * rep + h) * Tall;
-        for (int t = first + (int)threadIdx.x; t < last; t += 256) L[t] = -__builtin_inff();
-        if (qb * AT_QB >= T) return;  // uniform, before any barrier
-    }
     const uint16_t* Qp = Q + b * sqb + (int64_t)h * sqh;
     const uint16_t* Kp = K + b * skb + (int64_t)hk * skh;
     const uint16_t* Vp = V + b * svb + (int64_t)hk * svh;
@@ -248,9 +255,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     if (myq >= T) return;
     const float inv = 1.0f / lrun;
-    // one of the query's two lanes; the maximum in units of log 2, the sum's logarithm as one
-    if (LSE && hi == 0)
-        lse[((int64_t)b * Hkv * rep + h) * Tall + myq] = (mrun + __builtin_amdgcn_logf(lrun)) * 0.6931471805599453f;
     uint16_t* Op = O + b * sob + (int64_t)h * soh + (int64_t)myq * sot;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -267,14 +271,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
 }
 
-template <bool LSE>
-static int attention_launch(const uint16_t* q, int64_t sqb, int64_t sqh, int64_t sqt, const uint16_t* k, int64_t skb,
-                            int64_t skh, int64_t skt, const uint16_t* v, int64_t svb, int64_t svh, int64_t svt,
-                            uint16_t* out, int64_t sob, int64_t soh, int64_t sot, int64_t B, int64_t H, int64_t Hkv,
-                            int64_t T, int64_t D, float scale, const int32_t* lens, float* lse, void* stream)
+// out[b, t, h, :] = softmax(q[b, h, t, :] k[b, h / rep, :t + 1, :]^T * scale) v[b, h / rep, :t + 1, :], bf16 in and out;
+// every tensor's head dim (128) contiguous, the other strides in elements.
+extern "C" int lamq_attention_causal_bf16(const uint16_t* q, int64_t sqb, int64_t sqh, int64_t sqt, const uint16_t* k,
+                                          int64_t skb, int64_t skh, int64_t skt, const uint16_t* v, int64_t svb,
+                                          int64_t svh, int64_t svt, uint16_t* out, int64_t sob, int64_t soh,
+                                          int64_t sot, int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t D,
+                                          float scale, void* stream)
 {
-    if (!q || !k || !v || !out || (LSE && !lse) || B < 0 || H < 1 || Hkv < 1 || T < 0 || H % Hkv != 0)
-        return LAMQ_EINVAL;
+    if (!q || !k || !v || !out || B < 0 || H < 1 || Hkv < 1 || T < 0 || H % Hkv != 0) return LAMQ_EINVAL;
     if (D != AT_D) return LAMQ_EUNSUP;
     if (!(scale > 0.0f) || !(scale < 3.0e38f)) return LAMQ_EINVAL;
     const int64_t strides[12] = {sqb, sqh, sqt, skb, skh, skt, svb, svh, svt, sob, soh, sot};
@@ -287,31 +292,9 @@ static int attention_launch(const uint16_t* q, int64_t sqb, int64_t sqh, int64_t
     // a grid's work items along x must stay below 2^32, so past 2^22 workgroups they go out in rows
     const int64_t wgs = cdiv(T, AT_QB) * H * B, gx = wgs < AT_GRID_X ? wgs : AT_GRID_X;
     const dim3 grid((unsigned)gx, (unsigned)cdiv(wgs, gx));
-    hipLaunchKernelGGL(attention_causal_kernel<LSE>, grid, dim3(256), 0, as_stream(stream), q, sqb, sqh, sqt, k, skb, skh,
-                       skt, v, svb, svh, svt, out, sob, soh, sot, (int)(H / Hkv), (int)Hkv, (int)(B * Hkv), (int)T,
-                       scale * 1.4426950408889634f, lens, lse);
+    hipLaunchKernelGGL(attention_causal_kernel, grid, dim3(256), 0, as_stream(stream), q, sqb, sqh, sqt, k, skb, skh, skt,
+                       v, svb, svh, svt, out, sob, soh, sot, (int)(H / Hkv), (int)Hkv, (int)(B * Hkv), (int)T,
+                       scale * 1.4426950408889634f);
     LAMQ_LAUNCH_CHECK();
     return LAMQ_OK;
-}
-
-// out[b, t, h, :] = softmax(q[b, h, t, :] k[b, h / rep, :t + 1, :]^T * scale) v[b, h / rep, :t + 1, :], bf16 in and out;
-// every tensor's head dim (128) contiguous, the other strides in elements.
-extern "C" int lamq_attention_causal_bf16(const uint16_t* q, int64_t sqb, int64_t sqh, int64_t sqt, const uint16_t* k,
-                                          int64_t skb, int64_t skh, int64_t skt, const uint16_t* v, int64_t svb,
-                                          int64_t svh, int64_t svt, uint16_t* out, int64_t sob, int64_t soh,
-                                          int64_t sot, int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t D,
-                                          float scale, void* stream)
-{
-    return attention_launch<false>(q, sqb, sqh, sqt, k, skb, skh, skt, v, svb, svh, svt, out, sob, soh, sot, B, H, Hkv, T,
-                                   D, scale, nullptr, nullptr, stream);
-}
-
-// The same over the first lens[b] tokens of each sequence (lens NULL: all T), keeping the log-sum-exp of every query.
-extern "C" int lamq_attention_causal_lse_bf16(const lamq_heads* q, const lamq_heads* k, const lamq_heads* v,
-                                              const lamq_heads* out, float* lse, const int32_t* lens, int64_t B,
-                                              int64_t H, int64_t Hkv, int64_t T, int64_t D, float scale, void* stream)
-{
-    if (!q || !k || !v || !out) return LAMQ_EINVAL;
-    return attention_launch<true>(q->data, q->sb, q->sh, q->st, k->data, k->sb, k->sh, k->st, v->data, v->sb, v->sh,
-                                  v->st, out->data, out->sb, out->sh, out->st, B, H, Hkv, T, D, scale, lens, lse, stream);
 }

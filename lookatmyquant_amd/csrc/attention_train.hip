@@ -1,17 +1,21 @@
-// The backward pass of the causal grouped-query attention of training: the probabilities are recomputed from the
-// forward's log-sum-exp, tile by tile, and never reach memory.
+// The causal grouped-query attention of training: a forward that takes the sequences' lengths and keeps the log-sum-exp
+// of every query's scores, and the backward pass, which recomputes the probabilities from it tile by tile; they never
+// reach memory.
 //
-// With S = scale Q K^T over u <= t < len, P = exp(S - lse), O = P V and dO the gradient of O:
+// With S = scale Q K^T over u <= t < len, lse_t = log sum_u exp S_tu, P = exp(S - lse), O = P V and dO the gradient of O:
 //   delta_t = sum_d dO_td O_td,  dP = dO V^T,  dS = P (dP - delta),
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,  dK and dV summed over a key/value head's query heads.
 //
-// Two kernels, so that each gradient has one owner and its sums one order (no atomics): attention_dq_kernel owns 128
+// The forward owns 128 queries a workgroup and walks the keys with a running maximum and sum. The backward is two
+// kernels, so that each gradient has one owner and its sums one order (no atomics): attention_dq_kernel owns 128
 // queries and walks the keys up to them, forming S^T, dP^T and dQ^T += K^T dS^T; attention_dkdv_kernel owns 64 keys and
 // walks the query heads and queries from them on, forming S, dP, dV^T += dO^T P and dK^T += Q^T dS. Seven products where
 // five would do with one pass; the two formed twice cost less than a float32 dQ added up in memory (a read and a
 // write of 4 bytes per query, head dim and key block) and keep the results the same from run to run.
 //
-// The operand layouts are the forward's (32x32x16 bf16 MFMA): with the owned rows as columns of the result, S^T (or S)
+// Operand layouts (32x32x16 bf16 MFMA): A[m][k] has lane l holding m = l % 32 and k = 8 (l / 32) .. + 7; B[k][n] has lane
+// l holding n = l % 32 and the same k; the result has lane l holding column l % 32 and rows 8 (v / 4) + 4 (l / 32) + v % 4 of
+// register v. With the owned rows as columns of the result, S^T (or S)
 // and dP come out as the second product's B operand as they stand, and that product's A operand is the walked tile read
 // transposed (ds_read_b64_tr_b16) in the result's own order. A walked tile is read both ways, so its 16-byte chunks are
 // XOR-swizzled by at_f(row), the row's two low bit pairs exchanged: 16 rows at one chunk touch 16 different chunk
@@ -19,8 +23,69 @@
 //
 // P is rounded to bf16 for dV as the forward rounds it for O, dS to bf16 for dQ and dK, the operand type of the matrix
 // instructions; scores, dP, delta and every sum are float32, each gradient rounded once at its end.
-#include "attention.h"
+#include "common.h"
 
+typedef __bf16 lamq_at_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float lamq_at_f32x16 __attribute__((ext_vector_type(16)));
+typedef short lamq_at_s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) lamq_at_s4 lamq_at_lds_s4;
+typedef __attribute__((address_space(3))) const lamq_at_bf16x8 lamq_at_lds_frag;
+
+#define AT_GRID_X (1 << 22)
+#define AT_D 128                        // head dim
+#define AT_LOG2E 1.4426950408889634f
+
+// the larger of this lane's value and lane ^ 32's (one swap of the wave's halves, no LDS)
+__device__ __forceinline__ float at_max32(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float at_sum32(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// the length of sequence b, 0 .. T (all T without lengths)
+__device__ __forceinline__ int at_length(const int32_t* __restrict__ lens, int b, int T)
+{
+    if (!lens) return T;
+    const int n = __builtin_amdgcn_readfirstlane(lens[b]);
+    return n < 0 ? 0 : n < T ? n : T;
+}
+
+// zeros into rows first .. last - 1 of 128 bf16 at `row` (a workgroup of 256, eight bytes a lane: the alignment asked
+// of outputs)
+__device__ __forceinline__ void at_zero_rows(uint16_t* base, int64_t stride, int first, int last)
+{
+    for (int i = (int)threadIdx.x; i < (last - first) * (AT_D / 4); i += 256)
+        *reinterpret_cast<uint2*>(base + (int64_t)(first + i / (AT_D / 4)) * stride + 4 * (i % (AT_D / 4))) =
+            make_uint2(0u, 0u);
+}
+
+// One operand by its (batch, head, token) strides in elements, the head dim contiguous.
+struct AtView {
+    const uint16_t* p;
+    int64_t sb, sh, st;
+};
+struct AtOut {
+    uint16_t* p;
+    int64_t sb, sh, st;
+};
+
+// One direct global->LDS load (16 bytes a lane into m0 + 16 * lane) from a uniform address and a 32-bit byte offset a
+// lane; M0 saved and restored around it, with the wait state its write needs (load_lds16).
+__device__ __forceinline__ void at_load_lds16(const uint16_t* base, uint32_t off, uint32_t m)
+{
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(off), "s"(base), "s"(m)
+                 : "memory");
+}
+
+#define AG_LAZY 8.0f                  // log 2 of how far the forward's maximum may lag
 #define AG_R 32                       // rows a wave owns
 #define AG_W 64                       // rows of a walked block
 #define AG_OWN 128                    // queries a workgroup owns
@@ -63,8 +128,7 @@ __device__ __forceinline__ void ag_load_block(const uint16_t* block, int64_t st,
 __device__ __forceinline__ uint32_t ag_frag_base(int row, int hi) { return at_fsw(row, hi); }
 __device__ __forceinline__ lamq_at_bf16x8 ag_frag(uint32_t base, int j, uint32_t block)
 {
-    typedef __attribute__((address_space(3))) const lamq_at_bf16x8 lds_frag;
-    return *(lds_frag*)(uintptr_t)((base ^ (32u * j)) + block);
+    return *(lamq_at_lds_frag*)(uintptr_t)((base ^ (32u * j)) + block);
 }
 // A operand of a product over the walked rows: head dims 32 t + li, rows 32 hf + 16 mi + 4 hi + {0..3} and + 8 (the row
 // eight further on differs by 2 in at_f, the one sixteen further on not at all).
@@ -128,6 +192,129 @@ __device__ __forceinline__ bool ag_place(int pairs, int per, int& pair, int& rem
         rem = id % per;
     }
     return true;
+}
+
+// The forward: O and the log-sum-exp. Per block of 64 keys a wave forms S^T = K Q^T (two tiles of 32 keys x 32 queries),
+// the block's maxima, P = exp2(scale S - m) and O^T += V^T P^T. m is the running maximum as of the last time some query's
+// maximum had grown by more than 2^AG_LAZY: until then P is at most that, which bf16 and the float32 sums take as they
+// are, and the 64 products that rescale O are left out (with the exact maximum some query of 32 grows in most blocks).
+// The sums of a query's two lanes are added at the end. 4 x 32 heads x 2,048: 195 -> FWD us against the exact maximum and
+// 32 keys a step.
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_lse_kernel(
+    AtView Q, AtView K, AtView V, AtOut O, float* __restrict__ lse, const int32_t* __restrict__ lens, int rep, int Hkv,
+    int pairs, int Tall, float scale_log2)
+{
+    __shared__ __align__(256) uint8_t lds[2][2][AG_OPB];  // [buffer][K, V]
+    const int nqb = (Tall + AG_OWN - 1) / AG_OWN;
+    int pair, rem;
+    if (!ag_place(pairs, nqb * rep, pair, rem)) return;
+    const int qb = nqb - 1 - rem / rep;  // the longest query blocks first
+    const int b = pair / Hkv, hk = pair % Hkv, h = hk * rep + rem % rep;
+    const int lane = (int)(threadIdx.x & 63), wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int li = lane & 31, hi = lane >> 5;
+    const int T = at_length(lens, b, Tall);
+    uint16_t* Op = O.p + b * O.sb + (int64_t)h * O.sh;
+    float* L = lse + ((int64_t)b * Hkv * rep + h) * Tall;
+    const int own0 = qb * AG_OWN, own1 = own0 + AG_OWN < Tall ? own0 + AG_OWN : Tall;
+    if (own1 > T) {
+        const int first = own0 > T ? own0 : T;
+        at_zero_rows(Op, O.st, first, own1);
+        for (int t = first + (int)threadIdx.x; t < own1; t += 256) L[t] = -__builtin_inff();
+        if (own0 >= T) return;  // uniform, before any barrier
+    }
+    const int q0 = own0 + AG_R * wv, myq = q0 + li, qrow = myq < T ? myq : T - 1;
+    const uint16_t* Kp = K.p + b * K.sb + (int64_t)hk * K.sh;
+    const uint16_t* Vp = V.p + b * V.sb + (int64_t)hk * V.sh;
+    const uint32_t base = lds_addr(lds);
+    const int nblk = ((own1 < T ? own1 : T) - 1) / AG_W + 1;
+    const int my_last = q0 < T ? (q0 + AG_R < T ? q0 + AG_R : T) - 1 : -1;
+    auto load_block = [&](int kb) {
+        const uint32_t buf = base + (uint32_t)((kb & 1) * 2 * AG_OPB);
+        const int r0 = kb * AG_W;
+        ag_load_block(Kp + r0 * K.st, K.st, T - r0, wv, lane, buf);
+        ag_load_block(Vp + r0 * V.st, V.st, T - r0, wv, lane, buf + AG_OPB);
+    };
+    load_block(0);
+    lamq_at_bf16x8 qf[8];
+    {
+        const uint16_t* Qr = Q.p + b * Q.sb + (int64_t)h * Q.sh + (int64_t)qrow * Q.st + 8 * hi;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) qf[j] = ag_row8(Qr + 16 * j);
+    }
+    ag_settle(qf);
+    lamq_at_f32x16 o[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[t][v] = 0.0f;
+    float m = -__builtin_inff(), sum = 0.0f;  // in units of log 2; this lane's keys' part of the sum
+    for (int kb = 0; kb < nblk; ++kb) {
+        wait_vm<0>();     // this wave's loads of block kb have landed
+        __syncthreads();  // everyone's; the other buffer is free
+        if (kb + 1 < nblk) load_block(kb + 1);
+        const int k0 = kb * AG_W;
+        if (k0 > my_last) continue;  // uniform: this wave's queries end before these keys
+        uint32_t fb = base + (uint32_t)((kb & 1) * 2 * AG_OPB) + ag_frag_base(li, hi);
+        uint32_t tb = base + (uint32_t)((kb & 1) * 2 * AG_OPB) + AG_OPB + ag_tr_base(0, lane);
+        asm volatile("" : "+v"(fb), "+v"(tb));  // the fragments' addresses formed here, not kept around the loop
+        lamq_at_f32x16 s[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[hf][v] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+                s[hf] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_frag(fb, j, hf * AG_HALF), qf[j], s[hf], 0, 0, 0);
+        lamq_at_bf16x8 vf[2][2][4];  // V's fragments read under the softmax
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) vf[hf][mi][t] = ag_tr_frag(tb, mi, t, hf * AG_HALF);
+        if (k0 + AG_W - 1 > q0) {  // the causal mask, only where the block reaches past the wave's first query
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    s[hf][v] = k0 + 32 * hf + 8 * (v >> 2) + 4 * hi + (v & 3) <= myq ? s[hf][v] : -__builtin_inff();
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int v = 1; v < 32; ++v) mx = fmaxf(mx, s[v >> 4][v & 15]);
+        mx = at_max32(mx) * scale_log2;
+        if (__builtin_amdgcn_ballot_w64(mx > m + AG_LAZY)) {  // uniform
+            const float up = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - up);  // 0 at the first block
+            sum *= alpha;
+            m = up;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[t][v] *= alpha;
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            if (hf && k0 + 32 > my_last) break;  // uniform: past this wave's queries
+            lamq_at_bf16x8 pf[2];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[hf][v], scale_log2, -m));
+                sum += p;
+                pf[v >> 3][v & 7] = (__bf16)p;
+            }
+#pragma unroll
+            for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[hf][mi][t], pf[mi], o[t], 0, 0, 0);
+        }
+    }
+    if (myq >= T) return;
+    sum = at_sum32(sum);
+    ag_store_row(Op + (int64_t)myq * O.st, o, 1.0f / sum, hi);
+    if (hi == 0) L[myq] = (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
 // dQ, and per query the log-sum-exp in units of log 2 and delta for the other kernel (rows [B, H, T] of stats and
@@ -205,6 +392,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const int k0 = kb * AG_W;
         uint32_t fb = base + (uint32_t)((kb & 1) * 2 * AG_OPB) + ag_frag_base(li, hi);
         uint32_t tb = base + (uint32_t)((kb & 1) * 2 * AG_OPB) + ag_tr_base(0, lane);
+        asm volatile("" : "+v"(fb), "+v"(tb));  // the fragments' addresses formed here, not kept around the loop
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
             if (k0 + 32 * hf > my_last) continue;  // uniform: past this wave's queries
@@ -386,6 +574,52 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 }
 
+// A tensor by its strides: 16-byte loads of inputs, 8-byte stores of outputs, 64 rows within a 32-bit byte offset
+static int at_heads(const lamq_heads* x, int64_t T, int align)
+{
+    if (!x || !x->data || (uintptr_t)x->data % align) return LAMQ_EINVAL;
+    for (int64_t s : {x->sb, x->sh, x->st})
+        if (s < 0 || s % 8 != 0) return LAMQ_EINVAL;
+    return T > 1 && x->st > 0xffffff ? LAMQ_EUNSUP : LAMQ_OK;
+}
+
+static int at_sizes(int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t D, float scale)
+{
+    if (B < 0 || H < 1 || Hkv < 1 || T < 0 || H % Hkv != 0) return LAMQ_EINVAL;
+    if (D != AT_D) return LAMQ_EUNSUP;
+    if (!(scale > 0.0f) || !(scale < 3.0e38f)) return LAMQ_EINVAL;
+    if (B > 65535 || H > 65535 || T > 0x7fffff) return LAMQ_EUNSUP;
+    return cdiv(T, AG_KEYS) * H * B > 0x7fffffff ? LAMQ_EUNSUP : LAMQ_OK;
+}
+
+// a grid's work items along x must stay below 2^32, so past 2^22 workgroups they go out in rows
+static dim3 at_grid(int64_t wgs)
+{
+    const int64_t gx = wgs < AT_GRID_X ? wgs : AT_GRID_X;
+    return dim3((unsigned)gx, (unsigned)cdiv(wgs, gx));
+}
+
+static AtView at_view(const lamq_heads* x) { return AtView{x->data, x->sb, x->sh, x->st}; }
+static AtOut at_out(const lamq_heads* x) { return AtOut{x->data, x->sb, x->sh, x->st}; }
+
+extern "C" int lamq_attention_causal_lse_bf16(const lamq_heads* q, const lamq_heads* k, const lamq_heads* v,
+                                              const lamq_heads* out, float* lse, const int32_t* lens, int64_t B,
+                                              int64_t H, int64_t Hkv, int64_t T, int64_t D, float scale, void* stream)
+{
+    int rc = at_sizes(B, H, Hkv, T, D, scale);
+    for (const lamq_heads* x : {q, k, v})
+        if (rc == LAMQ_OK) rc = at_heads(x, T, 16);
+    if (rc == LAMQ_OK) rc = at_heads(out, T, 8);
+    if (rc != LAMQ_OK) return rc;
+    if (!lse) return LAMQ_EINVAL;
+    if (B == 0 || T == 0) return LAMQ_OK;
+    hipLaunchKernelGGL(attention_lse_kernel, at_grid(cdiv(T, AG_OWN) * H * B), dim3(256), 0, as_stream(stream), at_view(q),
+                       at_view(k), at_view(v), at_out(out), lse, lens, (int)(H / Hkv), (int)Hkv, (int)(B * Hkv), (int)T,
+                       scale * AT_LOG2E);
+    LAMQ_LAUNCH_CHECK();
+    return LAMQ_OK;
+}
+
 extern "C" size_t lamq_attention_causal_grad_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t T)
 {
     if (B < 1 || H < 1 || Hkv < 1 || T < 1) return 0;
@@ -399,42 +633,27 @@ extern "C" int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_h
                                                int64_t D, float scale, void* workspace, size_t workspace_bytes,
                                                void* stream)
 {
-    if (!q || !k || !v || !out || !lse || !dout || !dq || !dk || !dv) return LAMQ_EINVAL;
-    if (B < 0 || H < 1 || Hkv < 1 || T < 0 || H % Hkv != 0) return LAMQ_EINVAL;
-    if (D != AT_D) return LAMQ_EUNSUP;
-    if (!(scale > 0.0f) || !(scale < 3.0e38f)) return LAMQ_EINVAL;
-    const lamq_heads* all[8] = {q, k, v, out, dout, dq, dk, dv};
-    for (int i = 0; i < 8; ++i) {
-        const lamq_heads& x = *all[i];
-        if (!x.data || (uintptr_t)x.data % (i < 5 ? 16 : 8)) return LAMQ_EINVAL;  // 16-byte loads, 8-byte stores
-        for (int64_t s : {x.sb, x.sh, x.st})
-            if (s < 0 || s % 8 != 0) return LAMQ_EINVAL;
-        if (T > 1 && x.st > 0xffffff) return LAMQ_EUNSUP;  // 64 rows within a 32-bit byte offset
-    }
+    int rc = at_sizes(B, H, Hkv, T, D, scale);
+    for (const lamq_heads* x : {q, k, v, out, dout})
+        if (rc == LAMQ_OK) rc = at_heads(x, T, 16);
+    for (const lamq_heads* x : {dq, dk, dv})
+        if (rc == LAMQ_OK) rc = at_heads(x, T, 8);
+    if (rc != LAMQ_OK) return rc;
+    if (!lse) return LAMQ_EINVAL;
     if (B == 0 || T == 0) return LAMQ_OK;
-    if (B > 65535 || H > 65535 || T > 0x7fffff) return LAMQ_EUNSUP;
-    const int64_t qwgs = cdiv(T, AG_OWN) * H * B, kwgs = cdiv(T, AG_KEYS) * Hkv * B;
-    if (qwgs > 0x7fffffff || kwgs > 0x7fffffff) return LAMQ_EUNSUP;
     if (!workspace || (uintptr_t)workspace % 4 ||
         workspace_bytes < lamq_attention_causal_grad_workspace_size(B, H, Hkv, T))
         return LAMQ_EINVAL;
-    const AtView vq{q->data, q->sb, q->sh, q->st}, vk{k->data, k->sb, k->sh, k->st}, vv{v->data, v->sb, v->sh, v->st},
-        vo{out->data, out->sb, out->sh, out->st}, vd{dout->data, dout->sb, dout->sh, dout->st};
-    const AtOut oq{dq->data, dq->sb, dq->sh, dq->st}, ok{dk->data, dk->sb, dk->sh, dk->st},
-        ov{dv->data, dv->sb, dv->sh, dv->st};
     float* stats = reinterpret_cast<float*>(workspace);
     const int64_t nstats = B * H * T;
     hipStream_t s = as_stream(stream);
-    // a grid's work items along x must stay below 2^32, so past 2^22 workgroups they go out in rows
-    auto grid = [](int64_t wgs) {
-        const int64_t gx = wgs < AT_GRID_X ? wgs : AT_GRID_X;
-        return dim3((unsigned)gx, (unsigned)cdiv(wgs, gx));
-    };
-    hipLaunchKernelGGL(attention_dq_kernel, grid(qwgs), dim3(256), 0, s, vq, vk, vv, vo, vd, oq, lse, lens, stats, nstats,
-                       (int)(H / Hkv), (int)Hkv, (int)(B * Hkv), (int)T, scale, scale * AT_LOG2E);
+    hipLaunchKernelGGL(attention_dq_kernel, at_grid(cdiv(T, AG_OWN) * H * B), dim3(256), 0, s, at_view(q), at_view(k),
+                       at_view(v), at_view(out), at_view(dout), at_out(dq), lse, lens, stats, nstats, (int)(H / Hkv),
+                       (int)Hkv, (int)(B * Hkv), (int)T, scale, scale * AT_LOG2E);
     LAMQ_LAUNCH_CHECK();
-    hipLaunchKernelGGL(attention_dkdv_kernel, grid(kwgs), dim3(256), 0, s, vq, vk, vv, vd, ok, ov, lens, stats, nstats,
-                       (int)(H / Hkv), (int)Hkv, (int)(B * Hkv), (int)T, scale, scale * AT_LOG2E);
+    hipLaunchKernelGGL(attention_dkdv_kernel, at_grid(cdiv(T, AG_KEYS) * Hkv * B), dim3(256), 0, s, at_view(q), at_view(k),
+                       at_view(v), at_view(dout), at_out(dk), at_out(dv), lens, stats, nstats, (int)(H / Hkv), (int)Hkv,
+                       (int)(B * Hkv), (int)T, scale, scale * AT_LOG2E);
     LAMQ_LAUNCH_CHECK();
     return LAMQ_OK;
 }

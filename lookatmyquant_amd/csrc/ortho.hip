@@ -23,16 +23,50 @@ typedef _Float16 lamq_ns_f16x4 __attribute__((ext_vector_type(4)));
 typedef float lamq_ns_f32x16 __attribute__((ext_vector_type(16)));
 typedef short lamq_ns_s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) lamq_ns_s4 lamq_ns_lds_s4;
+typedef __attribute__((address_space(3))) const lamq_ns_f16x8 lamq_ns_lds_f16x8;
 
 #define NS_T 128                     // output tile
 #define NS_K 64                      // depth of a stage
 #define NS_OPB (NS_T * NS_K * 2)     // bytes of one operand's stage (16 KB)
+#define NS_CUS 256                   // compute units: up to as many tiles, one has a unit (and all its LDS) to itself
 #define NS_PARTS 256                 // partial sums of squares a matrix
 #define NS_SCALE 1024.0f             // what X, A and B are stored times
 #define NS_UNSCALE (1.0f / 1024.0f)
 
 __device__ __forceinline__ float ns_load(const float* p) { return *p; }
 __device__ __forceinline__ float ns_load(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
+
+// `m` (up to eight) entries at p, any alignment of the type, zeros past them
+typedef uint32_t lamq_ns_u4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float lamq_ns_f4 __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void ns_load8(const uint16_t* p, int m, float (&v)[8])
+{
+    if (m == 8) {
+        const lamq_ns_u4 x = *reinterpret_cast<const lamq_ns_u4*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(x[i] << 16);
+            v[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < m ? ns_load(p + i) : 0.0f;
+    }
+}
+__device__ __forceinline__ void ns_load8(const float* p, int m, float (&v)[8])
+{
+    if (m == 8) {
+        const lamq_ns_f4 x = reinterpret_cast<const lamq_ns_f4*>(p)[0], y = reinterpret_cast<const lamq_ns_f4*>(p)[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = x[i];
+            v[4 + i] = y[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < m ? ns_load(p + i) : 0.0f;
+    }
+}
 
 // The sum over the workgroup of 256, in every thread, in a fixed order.
 __device__ __forceinline__ double ns_sum(double x)
@@ -52,11 +86,26 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const Elt* __restrict__ G,
                                                       int64_t stride, double* __restrict__ parts)
 {
     const Elt* g = G + blockIdx.y * stride;
+    // by groups of eight columns of a row: whole 16-byte loads at any alignment of the type
     double x = 0.0;
-    const int64_t n = rows * cols;
-    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < n; i += 256 * (int64_t)gridDim.x) {
-        const double v = (double)ns_load(g + i / cols * ld + i % cols);
-        x += v * v;
+    const int64_t groups = (cols + 7) / 8, n = rows * groups;
+    int64_t i = blockIdx.x * 256 + threadIdx.x;
+    const int64_t by = 256 * (int64_t)gridDim.x;
+    int64_t r = i / groups, c = i % groups;
+    const int64_t br = by / groups, bc = by % groups;
+    for (; i < n; i += by) {
+        const Elt* p = g + r * ld + 8 * c;
+        const int m = (int)(cols - 8 * c < 8 ? cols - 8 * c : 8);
+        float v[8];
+        ns_load8(p, m, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x = fma((double)v[e], (double)v[e], x);
+        r += br;
+        c += bc;
+        if (c >= groups) {
+            c -= groups;
+            ++r;
+        }
     }
     x = ns_sum(x);
     if (threadIdx.x == 0) parts[blockIdx.y * gridDim.x + blockIdx.x] = x;
@@ -98,29 +147,48 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const Elt* __restrict__ G
     }
 }
 
-// One stage of an operand whose rows run along the product's depth: 128 rows of 64, 128 bytes a row in LDS, 16-byte
-// chunks XOR-swizzled by row / 2 % 8 (16 rows at one chunk then touch all 64 banks once). Wave wv's instruction q fills
-// rows 32 wv + 8 q .. + 7, lane l the slot l % 8 of row l / 8.
-__device__ __forceinline__ uint32_t ns_sw(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4)); }
-__device__ __forceinline__ void ns_stage(const uint16_t* P, int64_t ld, int k0, int wv, int lane, uint32_t buf)
+// Four direct global->LDS loads, 16 bytes a lane into m + 1024 q + 16 * lane, from uniform addresses and 32-bit byte
+// offsets a lane. M0 is written once, with the wait state its write needs (load_lds16), and restored: the loads' own
+// offset moves both addresses, so load q's uniform address is given 1024 q bytes short.
+__device__ __forceinline__ void ns_load4(const uint16_t* base, int64_t step, uint32_t o0, uint32_t o1, uint32_t m)
 {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int row = 32 * wv + 8 * q + (lane >> 3);
-        load_lds16(P + row * ld + k0 + 8 * ((lane & 7) ^ ((row >> 1) & 7)), buf + (uint32_t)((4 * wv + q) * 1024));
-    }
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %7\n\ts_nop 0\n\t"
+                 "global_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %4 offset:1024\n\t"
+                 "global_load_lds_dwordx4 %1, %5 offset:2048\n\tglobal_load_lds_dwordx4 %2, %6 offset:3072\n\t"
+                 "s_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(o0), "v"(o1), "s"(base), "s"(base + step - 512), "s"(base + 2 * step - 1024),
+                   "s"(base + 3 * step - 1536), "s"(m)
+                 : "memory");
 }
-// ... and of one whose rows are the depth: 64 rows of 128, 256 bytes a row, chunks swizzled by 4 (row % 4) for the
-// transposing reads (four rows by four chunks at a time).
-__device__ __forceinline__ uint32_t ns_tsw(int row, int chunk) { return (uint32_t)(row * 256 + ((chunk ^ (4 * (row & 3))) << 4)); }
-__device__ __forceinline__ void ns_stage_t(const uint16_t* P, int64_t ld, int k0, int wv, int lane, uint32_t buf)
+
+// One stage of an operand whose rows run along the product's depth: 128 rows of 64, 128 bytes a row in LDS, 16-byte
+// chunks XOR-swizzled by row / 2 % 8 (16 rows at one chunk then touch all 64 banks once). Wave wv's load q fills rows
+// 32 wv + 8 q .. + 7, lane l the slot l % 8 of row l / 8: chunk l % 8 ^ l / 16 ^ 4 (q % 2).
+__device__ __forceinline__ uint32_t ns_sw(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4)); }
+__device__ __forceinline__ uint32_t ns_off(int64_t ld, int lane)
 {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int row = 16 * wv + 4 * q + (lane >> 4);
-        load_lds16(P + (int64_t)(k0 + row) * ld + 8 * ((lane & 15) ^ (4 * (row & 3))),
-                   buf + (uint32_t)((4 * wv + q) * 1024));
-    }
+    return (uint32_t)(lane >> 3) * (uint32_t)(2 * ld) + 16u * (uint32_t)((lane & 7) ^ (lane >> 4));
+}
+__device__ __forceinline__ void ns_stage(const uint16_t* P, int64_t ld, uint32_t off, int wv, uint32_t buf)
+{
+    ns_load4(P + 32 * wv * ld, 8 * ld, off, off ^ 64u, buf + (uint32_t)(4096 * wv));
+}
+// ... and of one whose rows are the depth: 64 rows of 128, as two panels of 64 columns, 128 bytes a row. Chunks are
+// swizzled by 4 (row / 2 % 2) for the transposing reads (four rows by four chunks at a time). Wave wv's load q fills rows
+// 16 (wv % 2) + 8 q .. + 7 (q = 0, 1) and 32 further (q = 2, 3) of panel wv / 2.
+__device__ __forceinline__ uint32_t ns_toff(int64_t ld, int lane)
+{
+    return (uint32_t)(lane >> 3) * (uint32_t)(2 * ld) + 16u * (uint32_t)((lane & 7) ^ (4 * ((lane >> 4) & 1)));
+}
+__device__ __forceinline__ uint32_t ns_tsw(int row, int chunk)
+{
+    return (uint32_t)(row * 128 + ((chunk ^ (4 * ((row >> 1) & 1))) << 4));
+}
+__device__ __forceinline__ void ns_stage_t(const uint16_t* P, int64_t ld, uint32_t off, int wv, uint32_t buf)
+{
+    ns_load4(P + 64 * (wv >> 1) + 32 * (wv & 1) * ld, 8 * ld, off, off, buf + (uint32_t)(8192 * (wv >> 1) + 4096 * (wv & 1)));
 }
 
 enum NSMode { NS_GRAM, NS_POLY, NS_UPDATE, NS_LAST };
@@ -139,11 +207,11 @@ struct NSArgs {
 
 // C = P Q^T (gram, poly: lower tiles, each stored twice) or P Q (update): 128 x 128 tiles, four waves of 64 x 64, two
 // LDS stages filled by direct loads.
-template <int MODE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void ns_product_kernel(NSArgs g)
+template <int MODE, int RING>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING == 2 ? 2 : 1, 2))) void ns_product_kernel(NSArgs g)
 {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
-    __shared__ __align__(16) uint8_t lds[2][2][NS_OPB];
+    __shared__ __align__(256) uint8_t lds[RING][2][NS_OPB];
     const int lane = (int)(threadIdx.x & 63), wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int li = lane & 31, half = lane >> 5, grp = lane >> 4, i16 = lane & 15;
     const int64_t batch = blockIdx.y;
@@ -161,15 +229,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const uint16_t* P = g.p + batch * g.sp + (int64_t)I * NS_T * g.ldp;
     const uint16_t* Q = g.q + batch * g.sq + (SYM ? (int64_t)J * NS_T * g.ldq : (int64_t)J * NS_T);
     const uint32_t base = lds_addr(lds);
+    const uint32_t poff = ns_off(g.ldp, lane), qoff = SYM ? ns_off(g.ldq, lane) : ns_toff(g.ldq, lane);
     auto stage = [&](int st) {
-        const uint32_t buf = base + (uint32_t)((st & 1) * 2 * NS_OPB);
-        ns_stage(P, g.ldp, st * NS_K, wv, lane, buf);
+        const uint32_t buf = base + (uint32_t)((st % RING) * 2 * NS_OPB);
+        ns_stage(P + st * NS_K, g.ldp, poff, wv, buf);
         if (SYM)
-            ns_stage(Q, g.ldq, st * NS_K, wv, lane, buf + NS_OPB);
+            ns_stage(Q + st * NS_K, g.ldq, qoff, wv, buf + NS_OPB);
         else
-            ns_stage_t(Q, g.ldq, st * NS_K, wv, lane, buf + NS_OPB);
+            ns_stage_t(Q + (int64_t)st * NS_K * g.ldq, g.ldq, qoff, wv, buf + NS_OPB);
     };
     const int wm = 64 * (wv >> 1), wn = 64 * (wv & 1);
+    // LDS addresses of the fragments: chunk 2 ks + half of a row is the first one's address ^ 32 ks, 32 rows on the same
+    // 4,096 bytes on; read transposed, 16 rows are 2,048 bytes and 32 columns ^ 64
+    const uint32_t pbase = base + ns_sw(wm + li, half);
+    const uint32_t qbase = SYM ? base + NS_OPB + ns_sw(wn + li, half)
+                               : base + NS_OPB + (uint32_t)(8192 * (wn >> 6)) + ns_tsw(8 * half + (i16 >> 2), 2 * (grp & 1) + ((i16 & 3) >> 1)) +
+                                     8 * (i16 & 1);
     lamq_ns_f32x16 acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -178,29 +253,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
     const int nst = g.K / NS_K;
-    stage(0);
+#pragma unroll
+    for (int st = 0; st < RING - 1; ++st)
+        if (st < nst) stage(st);
     for (int st = 0; st < nst; ++st) {
-        wait_vm<0>();     // this wave's loads of the stage have landed
-        __syncthreads();  // everyone's; the other buffer is free
-        if (st + 1 < nst) stage(st + 1);
-        const uint8_t* pl = lds[st & 1][0];
-        const uint8_t* ql = lds[st & 1][1];
-        const uint32_t qb = base + (uint32_t)(((st & 1) * 2 + 1) * NS_OPB);
+        if (st + RING - 1 <= nst)
+            wait_vm<8 * (RING - 2)>();  // this wave's loads of the stage have landed, the later stages' may be under way
+        else
+            wait_vm<0>();
+        __syncthreads();  // everyone's; the buffer of the stage before is free
+        if (st + RING - 1 < nst) stage(st + RING - 1);
+        uint32_t pa = pbase + (uint32_t)((st % RING) * 2 * NS_OPB), qa = qbase + (uint32_t)((st % RING) * 2 * NS_OPB);
+        asm volatile("" : "+v"(pa), "+v"(qa));  // the fragments' addresses formed here, not kept around the loop
 #pragma unroll
         for (int ks = 0; ks < NS_K / 16; ++ks) {
             lamq_ns_f16x8 pf[2], qf[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                pf[i] = *reinterpret_cast<const lamq_ns_f16x8*>(pl + ns_sw(wm + 32 * i + li, 2 * ks + half));
+                pf[i] = *(lamq_ns_lds_f16x8*)(uintptr_t)((pa ^ (32u * ks)) + 4096u * i);
                 if (SYM) {
-                    qf[i] = *reinterpret_cast<const lamq_ns_f16x8*>(ql + ns_sw(wn + 32 * i + li, 2 * ks + half));
+                    qf[i] = *(lamq_ns_lds_f16x8*)(uintptr_t)((qa ^ (32u * ks)) + 4096u * i);
                 } else {
-                    // depth 16 ks + 8 half + {0..7} of column wn + 32 i + li: two transposing reads of four each
-                    const int row = 16 * ks + 8 * half + (i16 >> 2), col = wn + 32 * i + 16 * (grp & 1) + 4 * (i16 & 3);
-                    const uint32_t a0 = qb + ns_tsw(row, col >> 3) + 8 * ((col >> 2) & 1);
-                    const uint32_t a1 = qb + ns_tsw(row + 4, col >> 3) + 8 * ((col >> 2) & 1);
-                    const lamq_ns_s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)a0);
-                    const lamq_ns_s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)a1);
+                    // depth 16 ks + 8 half + {0..7} of column wn + 32 i + li: two transposing reads of four each, the second
+                    // four rows on (whose chunks are swizzled alike)
+                    const uint32_t at = (qa ^ (64u * i)) + 2048u * ks;
+                    const lamq_ns_s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)at);
+                    const lamq_ns_s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)(at + 512));
                     const short __attribute__((ext_vector_type(8))) x =
                         __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
                     qf[i] = __builtin_bit_cast(lamq_ns_f16x8, x);
@@ -390,14 +468,14 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
         y.sp = y.sq = p.mp * p.np;
         y.K = (int)p.np;
         y.out = A;
-        hipLaunchKernelGGL(ns_product_kernel<NS_GRAM>, lower, dim3(256), 0, st, y);
+        hipLaunchKernelGGL((lower.x * lower.y <= NS_CUS ? ns_product_kernel<NS_GRAM, 4> : ns_product_kernel<NS_GRAM, 2>), lower, dim3(256), 0, st, y);
         LAMQ_LAUNCH_CHECK();
         y.p = y.q = y.in_hi = A;
         y.ldp = y.ldq = p.mp;
         y.sp = y.sq = p.mp * p.mp;
         y.K = (int)p.mp;
         y.out = Bm;
-        hipLaunchKernelGGL(ns_product_kernel<NS_POLY>, lower, dim3(256), 0, st, y);
+        hipLaunchKernelGGL((lower.x * lower.y <= NS_CUS ? ns_product_kernel<NS_POLY, 4> : ns_product_kernel<NS_POLY, 2>), lower, dim3(256), 0, st, y);
         LAMQ_LAUNCH_CHECK();
         y.p = Bm;
         y.q = y.in_hi = hi[k & 1];
@@ -405,9 +483,9 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
         y.sq = p.mp * p.np;
         y.out = hi[1 - (k & 1)];
         if (k + 1 < steps)
-            hipLaunchKernelGGL(ns_product_kernel<NS_UPDATE>, full, dim3(256), 0, st, y);
+            hipLaunchKernelGGL((full.x * full.y <= NS_CUS ? ns_product_kernel<NS_UPDATE, 4> : ns_product_kernel<NS_UPDATE, 2>), full, dim3(256), 0, st, y);
         else
-            hipLaunchKernelGGL(ns_product_kernel<NS_LAST>, full, dim3(256), 0, st, y);
+            hipLaunchKernelGGL((full.x * full.y <= NS_CUS ? ns_product_kernel<NS_LAST, 4> : ns_product_kernel<NS_LAST, 2>), full, dim3(256), 0, st, y);
         LAMQ_LAUNCH_CHECK();
     }
     return LAMQ_OK;

@@ -253,66 +253,78 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING == 2 ?
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
     const int nst = g.K / NS_K;
+    // the fragments of step ks of the stage in buffer `buf`
+    auto frags = [&](int buf, int ks, lamq_ns_f16x8 (&pf)[2], lamq_ns_f16x8 (&qf)[2]) {
+        uint32_t pa = pbase + (uint32_t)(buf * 2 * NS_OPB), qa = qbase + (uint32_t)(buf * 2 * NS_OPB);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            pf[i] = *(lamq_ns_lds_f16x8*)(uintptr_t)((pa ^ (32u * ks)) + 4096u * i);
+            if (SYM) {
+                qf[i] = *(lamq_ns_lds_f16x8*)(uintptr_t)((qa ^ (32u * ks)) + 4096u * i);
+            } else {
+                // depth 16 ks + 8 half + {0..7} of column wn + 32 i + li: two transposing reads of four each, the second
+                // four rows on (whose chunks are swizzled alike)
+                const uint32_t at = (qa ^ (64u * i)) + 2048u * ks;
+                const lamq_ns_s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)at);
+                const lamq_ns_s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)(at + 512));
+                const short __attribute__((ext_vector_type(8))) x = __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
+                qf[i] = __builtin_bit_cast(lamq_ns_f16x8, x);
+            }
+        }
+    };
+    // a lane's four registers in a row are neighbours of a row of C: the operands exchanged
+    auto products = [&](lamq_ns_f16x8 (&pf)[2], lamq_ns_f16x8 (&qf)[2]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf[j], pf[i], acc[i][j], 0, 0, 0);
+    };
 #pragma unroll
     for (int st = 0; st < RING - 1; ++st)
         if (st < nst) stage(st);
+    lamq_ns_f16x8 pf[2][2], qf[2][2];
     for (int st = 0; st < nst; ++st) {
-        if (st + RING - 1 <= nst)
-            wait_vm<8 * (RING - 2)>();  // this wave's loads of the stage have landed, the later stages' may be under way
+        // with two stages a stage has landed when it begins; with four, so has the one after it, whose first fragments are
+        // read under this one's last products
+        if (RING == 4 && st + RING - 1 <= nst)
+            wait_vm<8>();  // the last stage asked for may be under way
         else
             wait_vm<0>();
-        __syncthreads();  // everyone's; the buffer of the stage before is free
+        __syncthreads();  // every wave's loads; the buffer of the stage before is free
         if (st + RING - 1 < nst) stage(st + RING - 1);
-        uint32_t pa = pbase + (uint32_t)((st % RING) * 2 * NS_OPB), qa = qbase + (uint32_t)((st % RING) * 2 * NS_OPB);
-        asm volatile("" : "+v"(pa), "+v"(qa));  // the fragments' addresses formed here, not kept around the loop
+        if (RING == 2 || st == 0) frags(st % RING, 0, pf[0], qf[0]);
 #pragma unroll
         for (int ks = 0; ks < NS_K / 16; ++ks) {
-            lamq_ns_f16x8 pf[2], qf[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                pf[i] = *(lamq_ns_lds_f16x8*)(uintptr_t)((pa ^ (32u * ks)) + 4096u * i);
-                if (SYM) {
-                    qf[i] = *(lamq_ns_lds_f16x8*)(uintptr_t)((qa ^ (32u * ks)) + 4096u * i);
-                } else {
-                    // depth 16 ks + 8 half + {0..7} of column wn + 32 i + li: two transposing reads of four each, the second
-                    // four rows on (whose chunks are swizzled alike)
-                    const uint32_t at = (qa ^ (64u * i)) + 2048u * ks;
-                    const lamq_ns_s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)at);
-                    const lamq_ns_s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)(at + 512));
-                    const short __attribute__((ext_vector_type(8))) x =
-                        __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
-                    qf[i] = __builtin_bit_cast(lamq_ns_f16x8, x);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    // gram and poly: the operands exchanged, so that a lane's four registers in a row are neighbours of
-                    // a row of the (symmetric) result; update: lane li holds row li of P's
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf[j], pf[i], acc[i][j], 0, 0, 0);
+            // the next step's fragments are read before this one's products, in that order
+            __builtin_amdgcn_sched_barrier(0);
+            if (ks + 1 < NS_K / 16)
+                frags(st % RING, ks + 1, pf[(ks + 1) & 1], qf[(ks + 1) & 1]);
+            else if (RING == 4 && st + 1 < nst)
+                frags((st + 1) % RING, 0, pf[0], qf[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            products(pf[ks & 1], qf[ks & 1]);
         }
     }
     // result: lane's row of C wm + 32 i + li, columns wn + 32 j + 8 r + 4 half + {0..3} in registers 4 r .. 4 r + 3
+    if constexpr (SYM) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int row = I * NS_T + wm + 32 * i + li;
+        for (int i = 0; i < 2; ++i) {
+            const int row = I * NS_T + wm + 32 * i + li;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int col = J * NS_T + wn + 32 * j + 8 * r + 4 * half;
-                float x[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * r + e] * NS_UNSCALE;
-                if (SYM) {
+                for (int r = 0; r < 4; ++r) {
+                    const int col = J * NS_T + wn + 32 * j + 8 * r + 4 * half;
                     const int64_t at = batch * g.mp * g.mp + (int64_t)row * g.mp + col;
-                    lamq_ns_f16x4 o;
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * r + e] * NS_UNSCALE;
                     if (MODE == NS_POLY) {
                         const lamq_ns_f16x4 A = *reinterpret_cast<const lamq_ns_f16x4*>(g.in_hi + at);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[e] = fmaf(g.b, (float)A[e], g.c * x[e]);
                     }
+                    lamq_ns_f16x4 o;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[e] = (_Float16)x[e];
                     *reinterpret_cast<lamq_ns_f16x4*>(g.out + at) = o;
@@ -324,31 +336,81 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING == 2 ?
                             t[(int64_t)e * g.mp] = __builtin_bit_cast(uint16_t, y);
                         }
                     }
-                } else {
-                    const int64_t at = batch * g.mp * g.np + (int64_t)row * g.np + col;
-                    const lamq_ns_f16x4 H = *reinterpret_cast<const lamq_ns_f16x4*>(g.in_hi + at);
-                    const lamq_ns_f16x4 L = *reinterpret_cast<const lamq_ns_f16x4*>(g.out_lo + at);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = fmaf(g.a, (float)H[e] + (float)L[e], x[e]);
-                    if (MODE == NS_UPDATE) {
-                        lamq_ns_f16x4 h, l;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            h[e] = (_Float16)x[e];
-                            l[e] = (_Float16)(x[e] - (float)h[e]);
-                        }
-                        *reinterpret_cast<lamq_ns_f16x4*>(g.out + at) = h;
-                        *reinterpret_cast<lamq_ns_f16x4*>(g.out_lo + at) = l;
-                    } else if (row < g.m) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (col + e < g.n) {
-                                const int64_t to = g.tall ? (int64_t)(col + e) * g.ldb + row : (int64_t)row * g.ldb + col + e;
-                                g.bf[batch * g.sb + to] = __builtin_bit_cast(uint16_t, (__bf16)(x[e] * NS_UNSCALE));
-                            }
-                    }
                 }
+        }
+    } else {
+        // through LDS (16 KB a wave, chunks of four floats swizzled by the row), so that X is read and written by rows of
+        // 128 bytes: eight lanes a row, eight columns a lane
+        const int r8 = lane >> 3, c8 = lane & 7;
+        const int64_t at0 = batch * g.mp * g.np + (int64_t)(I * NS_T + wm + r8) * g.np + J * NS_T + wn + 8 * c8;
+        lamq_ns_f16x8 H[8], L[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            H[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.in_hi + at0 + (int64_t)(8 * y) * g.np);
+            L[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.np);
+        }
+        __syncthreads();  // every wave's last stage is done with
+        float4* tile = reinterpret_cast<float4*>(lds) + wv * 1024;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 32 * i + li, chunk = 8 * j + 2 * r + half;
+                    tile[row * 16 + (chunk ^ (row & 15))] =
+                        make_float4(acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]);
+                }
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            const int row = 8 * y + r8;  // of the wave's 64
+            float4* t0 = tile + row * 16 + ((2 * c8) ^ (row & 15));
+            float4* t1 = tile + row * 16 + ((2 * c8 + 1) ^ (row & 15));
+            const float4 u = *t0, w = *t1;
+            float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = fmaf(g.a, (float)H[y][e] + (float)L[y][e], x[e] * NS_UNSCALE);
+            if constexpr (MODE == NS_UPDATE) {
+                lamq_ns_f16x8 h, l;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    h[e] = (_Float16)x[e];
+                    l[e] = (_Float16)(x[e] - (float)h[e]);
+                }
+                *reinterpret_cast<lamq_ns_f16x8*>(g.out + at0 + (int64_t)(8 * y) * g.np) = h;
+                *reinterpret_cast<lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.np) = l;
+            } else if (g.tall) {  // back where it was, to be read by columns
+                *t0 = make_float4(x[0], x[1], x[2], x[3]);
+                *t1 = make_float4(x[4], x[5], x[6], x[7]);
+            } else {
+                const int m = I * NS_T + wm + row, n = J * NS_T + wn + 8 * c8;
+                if (m < g.m)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (n + e < g.n)
+                            g.bf[batch * g.sb + (int64_t)m * g.ldb + n + e] =
+                                __builtin_bit_cast(uint16_t, (__bf16)(x[e] * NS_UNSCALE));
             }
+        }
+        if constexpr (MODE == NS_LAST) {
+            if (g.tall) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int c = 0; c < 16; c += 2) {
+                        const int row = 32 * i + li, chunk = c + half;
+                        const float4 u = tile[row * 16 + (chunk ^ (row & 15))];
+                        const float x[4] = {u.x, u.y, u.z, u.w};
+                        const int m = I * NS_T + wm + row, n = J * NS_T + wn + 4 * chunk;
+                        if (m < g.m)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (n + e < g.n)
+                                    g.bf[batch * g.sb + (int64_t)(n + e) * g.ldb + m] =
+                                        __builtin_bit_cast(uint16_t, (__bf16)(x[e] * NS_UNSCALE));
+                    }
+            }
+        }
     }
 }
 

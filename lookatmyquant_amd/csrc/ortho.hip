@@ -111,12 +111,12 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(const Elt* __restrict__ G,
     if (threadIdx.x == 0) parts[blockIdx.y * gridDim.x + blockIdx.x] = x;
 }
 
-// X = G / ||G|| (0 for a zero matrix) as hi + lo float16 parts, times 2^10, [mp][np] with zeros past G; a tall G
+// X = G / ||G|| (0 for a zero matrix) as hi + lo float16 parts, times 2^10, [mp][np], rows lx apart, zeros past G; a tall G
 // transposed. A workgroup takes 64 x 64 entries of X.
 template <typename Elt, bool TALL>
 __global__ __launch_bounds__(256) void ns_start_kernel(const Elt* __restrict__ G, int64_t rows, int64_t cols, int64_t ld,
                                                        int64_t stride, const double* __restrict__ parts, int nparts,
-                                                       int mp, int np, uint16_t* __restrict__ hi,
+                                                       int mp, int lx, uint16_t* __restrict__ hi,
                                                        uint16_t* __restrict__ lo)
 {
     __shared__ float tile[64][65];
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const Elt* __restrict__ G
     for (int y = threadIdx.x >> 6; y < 64; y += 4) {
         const float v = tile[y][x];
         const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
-        const int64_t at = batch * mp * np + (int64_t)(r0 + y) * np + c0 + x;
+        const int64_t at = (batch * mp + r0 + y) * (int64_t)lx + c0 + x;
         hi[at] = __builtin_bit_cast(uint16_t, h);
         lo[at] = __builtin_bit_cast(uint16_t, l);
     }
@@ -196,7 +196,7 @@ enum NSMode { NS_GRAM, NS_POLY, NS_UPDATE, NS_LAST };
 struct NSArgs {
     const uint16_t *p, *q;  // operands: p [..][K] rows of the output; q [..][K] columns (gram, poly) or [K][..] (update)
     int64_t ldp, ldq, sp, sq;
-    int K, tiles_m, tiles_n, np, mp;
+    int K, tiles_m, mp, lx, la;  // rows of X lx apart, of A and B la
     uint16_t *out, *out_lo;  // A, B or the next X's hi; lo (read and written in place)
     const uint16_t* in_hi;   // poly: A; update: X's hi
     float a, b, c;
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING == 2 ?
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int col = J * NS_T + wn + 32 * j + 8 * r + 4 * half;
-                    const int64_t at = batch * g.mp * g.mp + (int64_t)row * g.mp + col;
+                    const int64_t at = (batch * g.mp + row) * (int64_t)g.la + col;
                     float x[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * r + e] * NS_UNSCALE;
@@ -329,11 +329,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING == 2 ?
                     for (int e = 0; e < 4; ++e) o[e] = (_Float16)x[e];
                     *reinterpret_cast<lamq_ns_f16x4*>(g.out + at) = o;
                     if (I != J) {
-                        uint16_t* t = g.out + batch * g.mp * g.mp + (int64_t)col * g.mp + row;
+                        uint16_t* t = g.out + (batch * g.mp + col) * (int64_t)g.la + row;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const _Float16 y = o[e];  // a bit cast of the element itself would read the first one's bits
-                            t[(int64_t)e * g.mp] = __builtin_bit_cast(uint16_t, y);
+                            t[(int64_t)e * g.la] = __builtin_bit_cast(uint16_t, y);
                         }
                     }
                 }
@@ -342,12 +342,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING == 2 ?
         // through LDS (16 KB a wave, chunks of four floats swizzled by the row), so that X is read and written by rows of
         // 128 bytes: eight lanes a row, eight columns a lane
         const int r8 = lane >> 3, c8 = lane & 7;
-        const int64_t at0 = batch * g.mp * g.np + (int64_t)(I * NS_T + wm + r8) * g.np + J * NS_T + wn + 8 * c8;
+        const int64_t at0 = (batch * g.mp + I * NS_T + wm + r8) * (int64_t)g.lx + J * NS_T + wn + 8 * c8;
         lamq_ns_f16x8 H[8], L[8];
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
-            H[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.in_hi + at0 + (int64_t)(8 * y) * g.np);
-            L[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.np);
+            H[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.in_hi + at0 + (int64_t)(8 * y) * g.lx);
+            L[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.lx);
         }
         __syncthreads();  // every wave's last stage is done with
         float4* tile = reinterpret_cast<float4*>(lds) + wv * 1024;
@@ -377,8 +377,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING == 2 ?
                     h[e] = (_Float16)x[e];
                     l[e] = (_Float16)(x[e] - (float)h[e]);
                 }
-                *reinterpret_cast<lamq_ns_f16x8*>(g.out + at0 + (int64_t)(8 * y) * g.np) = h;
-                *reinterpret_cast<lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.np) = l;
+                *reinterpret_cast<lamq_ns_f16x8*>(g.out + at0 + (int64_t)(8 * y) * g.lx) = h;
+                *reinterpret_cast<lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.lx) = l;
             } else if (g.tall) {  // back where it was, to be read by columns
                 *t0 = make_float4(x[0], x[1], x[2], x[3]);
                 *t1 = make_float4(x[4], x[5], x[6], x[7]);
@@ -430,8 +430,8 @@ __global__ __launch_bounds__(256) void ns_copy_kernel(const Elt* __restrict__ G,
 }
 
 struct NSPlan {
-    int64_t m, n, mp, np;
-    size_t x, aa, total;  // bytes of one [mp][np] and [mp][mp] array over the batch, and of everything
+    int64_t m, n, mp, np, lx, la;
+    size_t x, aa, total;  // bytes of one [mp][lx] and [mp][la] array over the batch, and of everything
 };
 static NSPlan ns_plan(int64_t batch, int64_t rows, int64_t cols)
 {
@@ -440,8 +440,12 @@ static NSPlan ns_plan(int64_t batch, int64_t rows, int64_t cols)
     p.n = rows < cols ? cols : rows;
     p.mp = cdiv(p.m, NS_T) * NS_T;
     p.np = cdiv(p.n, NS_T) * NS_T;
-    p.x = (size_t)batch * p.mp * p.np * 2;
-    p.aa = (size_t)batch * p.mp * p.mp * 2;
+    // rows an odd number of 128 bytes apart: at a multiple of 256 the eight rows a load takes fall on few of the memory's
+    // channels
+    p.lx = p.np + 64;
+    p.la = p.mp + 64;
+    p.x = (size_t)batch * p.mp * p.lx * 2;
+    p.aa = (size_t)batch * p.mp * p.la * 2;
     p.total = (size_t)batch * NS_PARTS * sizeof(double) + 3 * p.x + 2 * p.aa;
     return p;
 }
@@ -501,17 +505,17 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
     const dim3 sg((unsigned)(p.np / 64), (unsigned)(p.mp / 64), (unsigned)batch);
     if (tall)
         hipLaunchKernelGGL((ns_start_kernel<Elt, true>), sg, dim3(256), 0, st, G, rows, cols, ld, stride, parts, nparts,
-                           (int)p.mp, (int)p.np, hi[0], lo);
+                           (int)p.mp, (int)p.lx, hi[0], lo);
     else
         hipLaunchKernelGGL((ns_start_kernel<Elt, false>), sg, dim3(256), 0, st, G, rows, cols, ld, stride, parts, nparts,
-                           (int)p.mp, (int)p.np, hi[0], lo);
+                           (int)p.mp, (int)p.lx, hi[0], lo);
     LAMQ_LAUNCH_CHECK();
     const int tm = (int)(p.mp / NS_T), tn = (int)(p.np / NS_T);
     NSArgs x{};
-    x.np = (int)p.np;
+    x.lx = (int)p.lx;
+    x.la = (int)p.la;
     x.mp = (int)p.mp;
     x.tiles_m = tm;
-    x.tiles_n = tn;
     x.a = a;
     x.b = b;
     x.c = c;
@@ -526,23 +530,23 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
     for (int k = 0; k < steps; ++k) {
         NSArgs y = x;
         y.p = y.q = hi[k & 1];
-        y.ldp = y.ldq = p.np;
-        y.sp = y.sq = p.mp * p.np;
+        y.ldp = y.ldq = p.lx;
+        y.sp = y.sq = p.mp * p.lx;
         y.K = (int)p.np;
         y.out = A;
         hipLaunchKernelGGL((lower.x * lower.y <= NS_CUS ? ns_product_kernel<NS_GRAM, 4> : ns_product_kernel<NS_GRAM, 2>), lower, dim3(256), 0, st, y);
         LAMQ_LAUNCH_CHECK();
         y.p = y.q = y.in_hi = A;
-        y.ldp = y.ldq = p.mp;
-        y.sp = y.sq = p.mp * p.mp;
+        y.ldp = y.ldq = p.la;
+        y.sp = y.sq = p.mp * p.la;
         y.K = (int)p.mp;
         y.out = Bm;
         hipLaunchKernelGGL((lower.x * lower.y <= NS_CUS ? ns_product_kernel<NS_POLY, 4> : ns_product_kernel<NS_POLY, 2>), lower, dim3(256), 0, st, y);
         LAMQ_LAUNCH_CHECK();
         y.p = Bm;
         y.q = y.in_hi = hi[k & 1];
-        y.ldq = p.np;
-        y.sq = p.mp * p.np;
+        y.ldq = p.lx;
+        y.sq = p.mp * p.lx;
         y.out = hi[1 - (k & 1)];
         if (k + 1 < steps)
             hipLaunchKernelGGL((full.x * full.y <= NS_CUS ? ns_product_kernel<NS_UPDATE, 4> : ns_product_kernel<NS_UPDATE, 2>), full, dim3(256), 0, st, y);

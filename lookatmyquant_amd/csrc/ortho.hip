@@ -147,48 +147,34 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const Elt* __restrict__ G
     }
 }
 
-// Four direct global->LDS loads, 16 bytes a lane into m + 1024 q + 16 * lane, from uniform addresses and 32-bit byte
-// offsets a lane. M0 is written once, with the wait state its write needs (load_lds16), and restored: the loads' own
-// offset moves both addresses, so load q's uniform address is given 1024 q bytes short.
-__device__ __forceinline__ void ns_load4(const uint16_t* base, int64_t step, uint32_t o0, uint32_t o1, uint32_t m)
+// One direct global->LDS load, 16 bytes a lane into m + 16 * lane, from a uniform address and a 32-bit byte offset a lane;
+// M0 saved and restored around it, with the wait state its write needs (load_lds16).
+__device__ __forceinline__ void ns_load_lds(const uint16_t* base, uint32_t off, uint32_t m)
 {
     uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %7\n\ts_nop 0\n\t"
-                 "global_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %4 offset:1024\n\t"
-                 "global_load_lds_dwordx4 %1, %5 offset:2048\n\tglobal_load_lds_dwordx4 %2, %6 offset:3072\n\t"
-                 "s_mov_b32 m0, %0"
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep)
-                 : "v"(o0), "v"(o1), "s"(base), "s"(base + step - 512), "s"(base + 2 * step - 1024),
-                   "s"(base + 3 * step - 1536), "s"(m)
+                 : "v"(off), "s"(base), "s"(m)
                  : "memory");
 }
 
-// One stage of an operand whose rows run along the product's depth: 128 rows of 64, 128 bytes a row in LDS, 16-byte
-// chunks XOR-swizzled by row / 2 % 8 (16 rows at one chunk then touch all 64 banks once). Wave wv's load q fills rows
-// 32 wv + 8 q .. + 7, lane l the slot l % 8 of row l / 8: chunk l % 8 ^ l / 16 ^ 4 (q % 2).
+// LDS layouts. An operand whose rows run along the product's depth: rows of 64 entries (128 bytes), 16-byte chunks
+// XOR-swizzled by row / 2 % 8 (16 rows at one chunk then touch all 64 banks once). One load takes eight rows, lane l the
+// slot l % 8 of row l / 8: chunk l % 8 ^ l / 16, ^ 4 in every other eight rows.
 __device__ __forceinline__ uint32_t ns_sw(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4)); }
 __device__ __forceinline__ uint32_t ns_off(int64_t ld, int lane)
 {
     return (uint32_t)(lane >> 3) * (uint32_t)(2 * ld) + 16u * (uint32_t)((lane & 7) ^ (lane >> 4));
 }
-__device__ __forceinline__ void ns_stage(const uint16_t* P, int64_t ld, uint32_t off, int wv, uint32_t buf)
-{
-    ns_load4(P + 32 * wv * ld, 8 * ld, off, off ^ 64u, buf + (uint32_t)(4096 * wv));
-}
-// ... and of one whose rows are the depth: 64 rows of 128, as two panels of 64 columns, 128 bytes a row. Chunks are
-// swizzled by 4 (row / 2 % 2) for the transposing reads (four rows by four chunks at a time). Wave wv's load q fills rows
-// 16 (wv % 2) + 8 q .. + 7 (q = 0, 1) and 32 further (q = 2, 3) of panel wv / 2.
-__device__ __forceinline__ uint32_t ns_toff(int64_t ld, int lane)
-{
-    return (uint32_t)(lane >> 3) * (uint32_t)(2 * ld) + 16u * (uint32_t)((lane & 7) ^ (4 * ((lane >> 4) & 1)));
-}
+// One whose rows are the depth: 64 rows, as two panels of 64 columns, 128 bytes a row; chunks swizzled by 4 (row / 2 % 2)
+// for the transposing reads (four rows by four chunks at a time).
 __device__ __forceinline__ uint32_t ns_tsw(int row, int chunk)
 {
     return (uint32_t)(row * 128 + ((chunk ^ (4 * ((row >> 1) & 1))) << 4));
 }
-__device__ __forceinline__ void ns_stage_t(const uint16_t* P, int64_t ld, uint32_t off, int wv, uint32_t buf)
+__device__ __forceinline__ uint32_t ns_toff(int64_t ld, int lane)
 {
-    ns_load4(P + 64 * (wv >> 1) + 32 * (wv & 1) * ld, 8 * ld, off, off, buf + (uint32_t)(8192 * (wv >> 1) + 4096 * (wv & 1)));
+    return (uint32_t)(lane >> 3) * (uint32_t)(2 * ld) + 16u * (uint32_t)((lane & 7) ^ (4 * ((lane >> 4) & 1)));
 }
 
 enum NSMode { NS_GRAM, NS_POLY, NS_UPDATE, NS_LAST };
@@ -205,14 +191,20 @@ struct NSArgs {
     int m, n, tall;
 };
 
-// C = P Q^T (gram, poly: lower tiles, each stored twice) or P Q (update): 128 x 128 tiles, four waves of 64 x 64, two
-// LDS stages filled by direct loads.
-template <int MODE, int RING>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING == 2 ? 2 : 1, 2))) void ns_product_kernel(NSArgs g)
+// C = P Q^T (gram, poly: lower tiles, each stored twice) or P Q (update, last): tiles of 64 MT x 128. Four waves multiply,
+// 32 MT x 64 each, fed from a ring of RING LDS stages; four more load, by direct global->LDS loads, and do nothing else: a
+// wave that issues its loads itself stands at them until the unit's queue has taken them, and its products with it (Gram
+// product of 9,728 x 2,560 99 -> 73 us).
+template <int MODE, int MT, int RING>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 2 ? 4 : 2))) void ns_product_kernel(NSArgs g)
 {
     constexpr bool SYM = MODE == NS_GRAM || MODE == NS_POLY;
-    __shared__ __align__(256) uint8_t lds[RING][2][NS_OPB];
-    const int lane = (int)(threadIdx.x & 63), wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    constexpr bool AHEAD = RING > 3;              // a stage's first fragments are read in the stage before
+    constexpr int PB = 64 * MT * 128;             // bytes of P's part of a stage
+    constexpr int STAGE = PB + NS_OPB;
+    constexpr int LOADS = 2 * MT + 4;             // a loading wave's loads of a stage
+    __shared__ __align__(256) uint8_t lds[RING * STAGE];
+    const int lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), wv = wave & 3;
     const int li = lane & 31, half = lane >> 5, grp = lane >> 4, i16 = lane & 15;
     const int64_t batch = blockIdx.y;
     const int id = (int)xcd_remap(blockIdx.x, gridDim.x);
@@ -226,90 +218,105 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING == 2 ?
         I = id % g.tiles_m;
         J = id / g.tiles_m;
     }
-    const uint16_t* P = g.p + batch * g.sp + (int64_t)I * NS_T * g.ldp;
-    const uint16_t* Q = g.q + batch * g.sq + (SYM ? (int64_t)J * NS_T * g.ldq : (int64_t)J * NS_T);
     const uint32_t base = lds_addr(lds);
-    const uint32_t poff = ns_off(g.ldp, lane), qoff = SYM ? ns_off(g.ldq, lane) : ns_toff(g.ldq, lane);
-    auto stage = [&](int st) {
-        const uint32_t buf = base + (uint32_t)((st % RING) * 2 * NS_OPB);
-        ns_stage(P + st * NS_K, g.ldp, poff, wv, buf);
-        if (SYM)
-            ns_stage(Q + st * NS_K, g.ldq, qoff, wv, buf + NS_OPB);
-        else
-            ns_stage_t(Q + (int64_t)st * NS_K * g.ldq, g.ldq, qoff, wv, buf + NS_OPB);
-    };
-    const int wm = 64 * (wv >> 1), wn = 64 * (wv & 1);
+    const int nst = g.K / NS_K;
+    if (wave >= 4) {  // uniform
+        const uint16_t* P = g.p + batch * g.sp;
+        const uint16_t* Q = g.q + batch * g.sq + (SYM ? (int64_t)J * NS_T * g.ldq : (int64_t)J * NS_T);
+        const uint32_t poff = ns_off(g.ldp, lane), qoff = SYM ? ns_off(g.ldq, lane) : ns_toff(g.ldq, lane);
+        auto stage = [&](int st) {
+            const uint32_t buf = base + (uint32_t)((st % RING) * STAGE);
+#pragma unroll
+            for (int q = 0; q < 2 * MT; ++q) {
+                const int r = 16 * MT * wv + 8 * q;  // of the tile; rows past the matrix (mp is a multiple of 128) read its last
+                const int row = I * 64 * MT + r < g.mp ? I * 64 * MT + r : g.mp - 8 - 8 * (1 - (q & 1));
+                ns_load_lds(P + row * g.ldp + st * NS_K, q & 1 ? poff ^ 64u : poff, buf + (uint32_t)(128 * r));
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (SYM)
+                    ns_load_lds(Q + (32 * wv + 8 * q) * g.ldq + st * NS_K, q & 1 ? qoff ^ 64u : qoff,
+                                buf + (uint32_t)(PB + 128 * (32 * wv + 8 * q)));
+                else
+                    ns_load_lds(Q + (st * NS_K + 32 * (wv & 1) + 8 * q) * g.ldq + 64 * (wv >> 1), qoff,
+                                buf + (uint32_t)(PB + 8192 * (wv >> 1) + 128 * (32 * (wv & 1) + 8 * q)));
+        };
+#pragma unroll
+        for (int st = 0; st < RING - 1; ++st)
+            if (st < nst) stage(st);
+        for (int st = 0; st < nst; ++st) {
+            // this wave's loads of the stage have landed (of the one after it too, where its fragments are read ahead)
+            if (RING > 2 && st + RING - 1 <= nst)
+                wait_vm<LOADS * (AHEAD ? RING - 3 : RING - 2)>();
+            else
+                wait_vm<0>();
+            __syncthreads();  // every wave's; the buffer of the stage before is free
+            if (st + RING - 1 < nst) stage(st + RING - 1);
+        }
+        __syncthreads();  // the multiplying waves' last stage is done with
+        return;
+    }
+    const int wm = 32 * MT * (wv >> 1), wn = 64 * (wv & 1);
     // LDS addresses of the fragments: chunk 2 ks + half of a row is the first one's address ^ 32 ks, 32 rows on the same
     // 4,096 bytes on; read transposed, 16 rows are 2,048 bytes and 32 columns ^ 64
     const uint32_t pbase = base + ns_sw(wm + li, half);
-    const uint32_t qbase = SYM ? base + NS_OPB + ns_sw(wn + li, half)
-                               : base + NS_OPB + (uint32_t)(8192 * (wn >> 6)) + ns_tsw(8 * half + (i16 >> 2), 2 * (grp & 1) + ((i16 & 3) >> 1)) +
+    const uint32_t qbase = SYM ? base + PB + ns_sw(wn + li, half)
+                               : base + PB + (uint32_t)(8192 * (wn >> 6)) + ns_tsw(8 * half + (i16 >> 2), 2 * (grp & 1) + ((i16 & 3) >> 1)) +
                                      8 * (i16 & 1);
-    lamq_ns_f32x16 acc[2][2];
+    lamq_ns_f32x16 acc[MT][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
-    const int nst = g.K / NS_K;
     // the fragments of step ks of the stage in buffer `buf`
-    auto frags = [&](int buf, int ks, lamq_ns_f16x8 (&pf)[2], lamq_ns_f16x8 (&qf)[2]) {
-        uint32_t pa = pbase + (uint32_t)(buf * 2 * NS_OPB), qa = qbase + (uint32_t)(buf * 2 * NS_OPB);
+    auto frags = [&](int buf, int ks, lamq_ns_f16x8 (&pf)[MT], lamq_ns_f16x8 (&qf)[2]) {
+        const uint32_t pa = pbase + (uint32_t)(buf * STAGE), qa = qbase + (uint32_t)(buf * STAGE);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            pf[i] = *(lamq_ns_lds_f16x8*)(uintptr_t)((pa ^ (32u * ks)) + 4096u * i);
+        for (int i = 0; i < MT; ++i) pf[i] = *(lamq_ns_lds_f16x8*)(uintptr_t)((pa ^ (32u * ks)) + 4096u * i);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
             if (SYM) {
-                qf[i] = *(lamq_ns_lds_f16x8*)(uintptr_t)((qa ^ (32u * ks)) + 4096u * i);
+                qf[j] = *(lamq_ns_lds_f16x8*)(uintptr_t)((qa ^ (32u * ks)) + 4096u * j);
             } else {
-                // depth 16 ks + 8 half + {0..7} of column wn + 32 i + li: two transposing reads of four each, the second
+                // depth 16 ks + 8 half + {0..7} of column wn + 32 j + li: two transposing reads of four each, the second
                 // four rows on (whose chunks are swizzled alike)
-                const uint32_t at = (qa ^ (64u * i)) + 2048u * ks;
+                const uint32_t at = (qa ^ (64u * j)) + 2048u * ks;
                 const lamq_ns_s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)at);
                 const lamq_ns_s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lamq_ns_lds_s4*)(uintptr_t)(at + 512));
                 const short __attribute__((ext_vector_type(8))) x = __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
-                qf[i] = __builtin_bit_cast(lamq_ns_f16x8, x);
+                qf[j] = __builtin_bit_cast(lamq_ns_f16x8, x);
             }
         }
     };
-    // a lane's four registers in a row are neighbours of a row of C: the operands exchanged
-    auto products = [&](lamq_ns_f16x8 (&pf)[2], lamq_ns_f16x8 (&qf)[2]) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf[j], pf[i], acc[i][j], 0, 0, 0);
-    };
-#pragma unroll
-    for (int st = 0; st < RING - 1; ++st)
-        if (st < nst) stage(st);
-    lamq_ns_f16x8 pf[2][2], qf[2][2];
+    lamq_ns_f16x8 pf[2][MT], qf[2][2];
     for (int st = 0; st < nst; ++st) {
-        // with two stages a stage has landed when it begins; with four, so has the one after it, whose first fragments are
-        // read under this one's last products
-        if (RING == 4 && st + RING - 1 <= nst)
-            wait_vm<8>();  // the last stage asked for may be under way
-        else
-            wait_vm<0>();
-        __syncthreads();  // every wave's loads; the buffer of the stage before is free
-        if (st + RING - 1 < nst) stage(st + RING - 1);
-        if (RING == 2 || st == 0) frags(st % RING, 0, pf[0], qf[0]);
+        __syncthreads();  // the stage has landed
+        if (!AHEAD || st == 0) frags(st % RING, 0, pf[0], qf[0]);
 #pragma unroll
         for (int ks = 0; ks < NS_K / 16; ++ks) {
             // the next step's fragments are read before this one's products, in that order
             __builtin_amdgcn_sched_barrier(0);
             if (ks + 1 < NS_K / 16)
                 frags(st % RING, ks + 1, pf[(ks + 1) & 1], qf[(ks + 1) & 1]);
-            else if (RING == 4 && st + 1 < nst)
+            else if (AHEAD && st + 1 < nst)
                 frags((st + 1) % RING, 0, pf[0], qf[0]);
             __builtin_amdgcn_sched_barrier(0);
-            products(pf[ks & 1], qf[ks & 1]);
+            // a lane's four registers in a row are neighbours of a row of C: the operands exchanged
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qf[ks & 1][j], pf[ks & 1][i], acc[i][j], 0, 0, 0);
         }
     }
+    __syncthreads();  // every wave's last stage is done with
     // result: lane's row of C wm + 32 i + li, columns wn + 32 j + 8 r + 4 half + {0..3} in registers 4 r .. 4 r + 3
     if constexpr (SYM) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = I * NS_T + wm + 32 * i + li;
+        for (int i = 0; i < MT; ++i) {
+            const int row = I * 64 * MT + wm + 32 * i + li;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -341,74 +348,78 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(RING == 2 ?
     } else {
         // through LDS (16 KB a wave, chunks of four floats swizzled by the row), so that X is read and written by rows of
         // 128 bytes: eight lanes a row, eight columns a lane
-        const int r8 = lane >> 3, c8 = lane & 7;
-        const int64_t at0 = (batch * g.mp + I * NS_T + wm + r8) * (int64_t)g.lx + J * NS_T + wn + 8 * c8;
-        lamq_ns_f16x8 H[8], L[8];
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-            H[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.in_hi + at0 + (int64_t)(8 * y) * g.lx);
-            L[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.lx);
-        }
-        __syncthreads();  // every wave's last stage is done with
-        float4* tile = reinterpret_cast<float4*>(lds) + wv * 1024;
+        for (int h = 0; h < MT / 2; ++h) {  // 64 rows at a time
+            const int m0 = I * 64 * MT + wm + 64 * h;
+            if (m0 >= g.mp) break;  // uniform: past the matrix
+            const int r8 = lane >> 3, c8 = lane & 7;
+            const int64_t at0 = (batch * g.mp + m0 + r8) * (int64_t)g.lx + J * NS_T + wn + 8 * c8;
+            lamq_ns_f16x8 H[8], L[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 32 * i + li, chunk = 8 * j + 2 * r + half;
-                    tile[row * 16 + (chunk ^ (row & 15))] =
-                        make_float4(acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]);
-                }
-#pragma unroll
-        for (int y = 0; y < 8; ++y) {
-            const int row = 8 * y + r8;  // of the wave's 64
-            float4* t0 = tile + row * 16 + ((2 * c8) ^ (row & 15));
-            float4* t1 = tile + row * 16 + ((2 * c8 + 1) ^ (row & 15));
-            const float4 u = *t0, w = *t1;
-            float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = fmaf(g.a, (float)H[y][e] + (float)L[y][e], x[e] * NS_UNSCALE);
-            if constexpr (MODE == NS_UPDATE) {
-                lamq_ns_f16x8 h, l;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    h[e] = (_Float16)x[e];
-                    l[e] = (_Float16)(x[e] - (float)h[e]);
-                }
-                *reinterpret_cast<lamq_ns_f16x8*>(g.out + at0 + (int64_t)(8 * y) * g.lx) = h;
-                *reinterpret_cast<lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.lx) = l;
-            } else if (g.tall) {  // back where it was, to be read by columns
-                *t0 = make_float4(x[0], x[1], x[2], x[3]);
-                *t1 = make_float4(x[4], x[5], x[6], x[7]);
-            } else {
-                const int m = I * NS_T + wm + row, n = J * NS_T + wn + 8 * c8;
-                if (m < g.m)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (n + e < g.n)
-                            g.bf[batch * g.sb + (int64_t)m * g.ldb + n + e] =
-                                __builtin_bit_cast(uint16_t, (__bf16)(x[e] * NS_UNSCALE));
+            for (int y = 0; y < 8; ++y) {
+                H[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.in_hi + at0 + (int64_t)(8 * y) * g.lx);
+                L[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.lx);
             }
-        }
-        if constexpr (MODE == NS_LAST) {
-            if (g.tall) {
+            float4* tile = reinterpret_cast<float4*>(lds) + wv * 1024;
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int c = 0; c < 16; c += 2) {
-                        const int row = 32 * i + li, chunk = c + half;
-                        const float4 u = tile[row * 16 + (chunk ^ (row & 15))];
-                        const float x[4] = {u.x, u.y, u.z, u.w};
-                        const int m = I * NS_T + wm + row, n = J * NS_T + wn + 4 * chunk;
-                        if (m < g.m)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (n + e < g.n)
-                                    g.bf[batch * g.sb + (int64_t)(n + e) * g.ldb + m] =
-                                        __builtin_bit_cast(uint16_t, (__bf16)(x[e] * NS_UNSCALE));
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = 32 * i + li, chunk = 8 * j + 2 * r + half, a = 2 * h + i;
+                        tile[row * 16 + (chunk ^ (row & 15))] =
+                            make_float4(acc[a][j][4 * r], acc[a][j][4 * r + 1], acc[a][j][4 * r + 2], acc[a][j][4 * r + 3]);
                     }
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                const int row = 8 * y + r8;  // of the wave's 64
+                float4* t0 = tile + row * 16 + ((2 * c8) ^ (row & 15));
+                float4* t1 = tile + row * 16 + ((2 * c8 + 1) ^ (row & 15));
+                const float4 u = *t0, w = *t1;
+                float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = fmaf(g.a, (float)H[y][e] + (float)L[y][e], x[e] * NS_UNSCALE);
+                if constexpr (MODE == NS_UPDATE) {
+                    lamq_ns_f16x8 hv, lv;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        hv[e] = (_Float16)x[e];
+                        lv[e] = (_Float16)(x[e] - (float)hv[e]);
+                    }
+                    *reinterpret_cast<lamq_ns_f16x8*>(g.out + at0 + (int64_t)(8 * y) * g.lx) = hv;
+                    *reinterpret_cast<lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.lx) = lv;
+                } else if (g.tall) {  // back where it was, to be read by columns
+                    *t0 = make_float4(x[0], x[1], x[2], x[3]);
+                    *t1 = make_float4(x[4], x[5], x[6], x[7]);
+                } else {
+                    const int m = m0 + row, n = J * NS_T + wn + 8 * c8;
+                    if (m < g.m)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (n + e < g.n)
+                                g.bf[batch * g.sb + (int64_t)m * g.ldb + n + e] =
+                                    __builtin_bit_cast(uint16_t, (__bf16)(x[e] * NS_UNSCALE));
+                }
+            }
+            if constexpr (MODE == NS_LAST) {
+                if (g.tall) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int c = 0; c < 16; c += 2) {
+                            const int row = 32 * i + li, chunk = c + half;
+                            const float4 u = tile[row * 16 + (chunk ^ (row & 15))];
+                            const float x[4] = {u.x, u.y, u.z, u.w};
+                            const int m = m0 + row, n = J * NS_T + wn + 4 * chunk;
+                            if (m < g.m)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (n + e < g.n)
+                                        g.bf[batch * g.sb + (int64_t)(n + e) * g.ldb + m] =
+                                            __builtin_bit_cast(uint16_t, (__bf16)(x[e] * NS_UNSCALE));
+                        }
+                }
             }
         }
     }
@@ -515,7 +526,6 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
     x.lx = (int)p.lx;
     x.la = (int)p.la;
     x.mp = (int)p.mp;
-    x.tiles_m = tm;
     x.a = a;
     x.b = b;
     x.c = c;
@@ -526,7 +536,12 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
     x.m = (int)p.m;
     x.n = (int)p.n;
     x.tall = tall;
-    const dim3 lower((unsigned)(tm * (tm + 1) / 2), (unsigned)batch), full((unsigned)(tm * tn), (unsigned)batch);
+    const dim3 lower((unsigned)(tm * (tm + 1) / 2), (unsigned)batch);
+    // a ring of four stages (all of a unit's LDS) where every tile has a unit to itself, two where two tiles share one;
+    // updates of more tiles than units by tiles of 256 rows: UPDATE_NOTE
+    const bool alone = (int64_t)lower.x * batch <= NS_CUS, wide = (int64_t)tm * tn * batch > NS_CUS;
+    x.tiles_m = wide ? (tm + 1) / 2 : tm;
+    const dim3 full((unsigned)(x.tiles_m * tn), (unsigned)batch), wg(512);
     for (int k = 0; k < steps; ++k) {
         NSArgs y = x;
         y.p = y.q = hi[k & 1];
@@ -534,14 +549,14 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
         y.sp = y.sq = p.mp * p.lx;
         y.K = (int)p.np;
         y.out = A;
-        hipLaunchKernelGGL((lower.x * lower.y <= NS_CUS ? ns_product_kernel<NS_GRAM, 4> : ns_product_kernel<NS_GRAM, 2>), lower, dim3(256), 0, st, y);
+        hipLaunchKernelGGL((alone ? ns_product_kernel<NS_GRAM, 2, 4> : ns_product_kernel<NS_GRAM, 2, 2>), lower, wg, 0, st, y);
         LAMQ_LAUNCH_CHECK();
         y.p = y.q = y.in_hi = A;
         y.ldp = y.ldq = p.la;
         y.sp = y.sq = p.mp * p.la;
         y.K = (int)p.mp;
         y.out = Bm;
-        hipLaunchKernelGGL((lower.x * lower.y <= NS_CUS ? ns_product_kernel<NS_POLY, 4> : ns_product_kernel<NS_POLY, 2>), lower, dim3(256), 0, st, y);
+        hipLaunchKernelGGL((alone ? ns_product_kernel<NS_POLY, 2, 4> : ns_product_kernel<NS_POLY, 2, 2>), lower, wg, 0, st, y);
         LAMQ_LAUNCH_CHECK();
         y.p = Bm;
         y.q = y.in_hi = hi[k & 1];
@@ -549,9 +564,11 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
         y.sq = p.mp * p.lx;
         y.out = hi[1 - (k & 1)];
         if (k + 1 < steps)
-            hipLaunchKernelGGL((full.x * full.y <= NS_CUS ? ns_product_kernel<NS_UPDATE, 4> : ns_product_kernel<NS_UPDATE, 2>), full, dim3(256), 0, st, y);
+            hipLaunchKernelGGL((wide ? ns_product_kernel<NS_UPDATE, 4, 3> : ns_product_kernel<NS_UPDATE, 2, 4>), full, wg, 0,
+                               st, y);
         else
-            hipLaunchKernelGGL((full.x * full.y <= NS_CUS ? ns_product_kernel<NS_LAST, 4> : ns_product_kernel<NS_LAST, 2>), full, dim3(256), 0, st, y);
+            hipLaunchKernelGGL((wide ? ns_product_kernel<NS_LAST, 4, 3> : ns_product_kernel<NS_LAST, 2, 4>), full, wg, 0, st,
+                               y);
         LAMQ_LAUNCH_CHECK();
     }
     return LAMQ_OK;

@@ -29,6 +29,8 @@ typedef __attribute__((address_space(3))) const lamq_ns_f16x8 lamq_ns_lds_f16x8;
 #define NS_K 64                      // depth of a stage
 #define NS_OPB (NS_T * NS_K * 2)     // bytes of one operand's stage (16 KB)
 #define NS_CUS 256                   // compute units: up to as many tiles, one has a unit (and all its LDS) to itself
+#define NS_SMALL_M 128               // a matrix up to this goes through in one workgroup, whole
+#define NS_SMALL_N 512
 #define NS_PARTS 256                 // partial sums of squares a matrix
 #define NS_SCALE 1024.0f             // what X, A and B are stored times
 #define NS_UNSCALE (1.0f / 1024.0f)
@@ -425,6 +427,232 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
     }
 }
 
+// A small matrix, whole: m <= 128, n <= 512. One workgroup of 16 waves holds X in LDS as float16 (what the products
+// read) and, each wave 32 columns of it, in its accumulators as float32 times 2^10 (what a X takes), A and then B in
+// LDS; from G to the result nothing else goes through memory, and all steps are one launch. 128 x 320: 100 us by the
+// products above (17 launches of about 6 us, latencies all of it), 49 us here.
+__device__ __forceinline__ int ns_f(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }  // conflict-free both ways
+__device__ __forceinline__ uint32_t ns_xat(int row, int chunk)  // 16-byte chunk of X's row in LDS
+{
+    return (uint32_t)(row * (2 * NS_SMALL_N) + ((chunk ^ ns_f(row)) << 4));
+}
+__device__ __forceinline__ uint32_t ns_aat(int row, int chunk)  // and of A's
+{
+    return (uint32_t)(row * (2 * NS_SMALL_M) + ((chunk ^ ns_f(row)) << 4));
+}
+// four entries at p, any alignment of the type
+typedef uint32_t lamq_ns_u2 __attribute__((ext_vector_type(2), aligned(2)));
+__device__ __forceinline__ void ns_load4(const uint16_t* p, float (&v)[4])
+{
+    const lamq_ns_u2 x = *reinterpret_cast<const lamq_ns_u2*>(p);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        v[2 * i] = __uint_as_float(x[i] << 16);
+        v[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
+    }
+}
+__device__ __forceinline__ void ns_load4(const float* p, float (&v)[4])
+{
+    const lamq_ns_f4 x = *reinterpret_cast<const lamq_ns_f4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = x[i];
+}
+// ENTRIES: G and the result an entry a lane (a tall G, whose rows are X's columns, or rows of fewer than four), else by rows.
+template <typename Elt, bool ENTRIES>
+__global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ G, int64_t ld, int64_t stride,
+                                                        uint16_t* __restrict__ out, int64_t ldo, int64_t so, int m, int n,
+                                                        int tall, int steps, float a, float b, float c)
+{
+    __shared__ __align__(256) uint8_t xs[NS_SMALL_M * NS_SMALL_N * 2];
+    __shared__ __align__(256) uint8_t as[NS_SMALL_M * NS_SMALL_M * 2];
+    typedef __attribute__((address_space(3))) lamq_ns_f16x4 lds_f16x4;
+    const int lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    int li = lane & 31, half = lane >> 5, i16 = lane & 15;
+    const int mt = (m + 31) / 32, nt = (n + 31) / 32;  // tiles of 32
+    const uint32_t xb = lds_addr(xs), ab = lds_addr(as);
+    G += blockIdx.x * stride;
+    out += blockIdx.x * so;
+    const int c0 = 32 * wave + 4 * half;  // X's rows 32 i + li, columns c0 + 8 r + {0..3}
+    lamq_ns_f32x16 X[4];
+    double ss = 0.0;
+    // No load is conditional (a branch would wait for each in turn): past the matrix the address is held inside it and the
+    // value left out.
+    if constexpr (ENTRIES) {
+        const int64_t sr = tall ? 1 : ld, sc = tall ? ld : 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 32 * i + li;
+            const Elt* g = G + (row < m ? row : m - 1) * sr;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int col = c0 + 8 * (v >> 2) + (v & 3);
+                X[i][v] = ns_load(g + (col < n ? col : n - 1) * sc);
+            }
+        }
+    } else {
+        // eight lanes a row of 32 columns, then into the lanes' own places through LDS, 64 rows (8 KB a wave) at a time
+        const int cc = 32 * wave + 4 * (lane & 7), at = cc < n - 4 ? cc : n - 4, shift = cc - at;  // past the row by `shift`
+        float4* t = reinterpret_cast<float4*>(xs) + 512 * wave;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            __builtin_amdgcn_sched_barrier(0);
+            float x[8][4];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int row = 64 * h + 8 * q + (lane >> 3);
+                ns_load4(G + (row < m ? row : m - 1) * ld + at, x[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int y = 8 * q + (lane >> 3);
+                const float s0 = shift & 1 ? x[q][1] : x[q][0], s1 = shift & 1 ? x[q][2] : x[q][1],
+                            s2 = shift & 1 ? x[q][3] : x[q][2], s3 = x[q][3];
+                // (what moves past the end is left out below, whatever it is)
+                t[8 * y + ((lane & 7) ^ (y & 7))] = make_float4(shift & 2 ? s2 : s0, shift & 2 ? s3 : s1, s2, s3);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int y = 32 * i + li;
+                    const float4 v = t[8 * y + ((2 * r + half) ^ (y & 7))];
+                    X[2 * h + i][4 * r] = v.x;
+                    X[2 * h + i][4 * r + 1] = v.y;
+                    X[2 * h + i][4 * r + 2] = v.z;
+                    X[2 * h + i][4 * r + 3] = v.w;
+                }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            X[i][v] = 32 * i + li < m && c0 + 8 * (v >> 2) + (v & 3) < n ? X[i][v] : 0.0f;
+            ss = fma((double)X[i][v], (double)X[i][v], ss);
+        }
+    {
+        double* sums = reinterpret_cast<double*>(as);
+        for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o);
+        if (lane == 0) sums[wave] = ss;
+        __syncthreads();
+        ss = 0.0;
+        for (int w = 0; w < 16; ++w) ss += sums[w];
+    }
+    const double f = ss > 0.0 ? (double)NS_SCALE / sqrt(ss) : ss;  // NaN stays
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) X[i][v] = (float)((double)X[i][v] * f);
+    const int ti = wave >> 2, tj = wave & 3;  // this wave's tile of A and B
+    const bool mine = ti < mt && tj < mt, cols = wave < nt;  // uniform
+    for (int step = 0; step < steps; ++step) {
+        asm volatile("" : "+v"(li), "+v"(half), "+v"(i16));  // addresses are formed where they are used, not kept around the loop
+        if (cols)  // X as float16
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < mt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        lamq_ns_f16x4 h;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) h[e] = (_Float16)X[i][4 * r + e];
+                        *(lds_f16x4*)(uintptr_t)(xb + ns_xat(32 * i + li, 4 * wave + r) + 8 * half) = h;
+                    }
+        __syncthreads();  // X is there; B of the step before (and the sums) are read
+        lamq_ns_f32x16 T;
+        auto at = [&](int r) { return (lds_f16x4*)(uintptr_t)(ab + ns_aat(32 * ti + li, 4 * tj + r) + 8 * half); };
+        if (mine) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) T[v] = 0.0f;
+#pragma unroll 2
+            for (int ks = 0; ks < 2 * nt; ++ks) {
+                const lamq_ns_f16x8 p = *(lamq_ns_lds_f16x8*)(uintptr_t)(xb + ns_xat(32 * ti + li, 2 * ks + half));
+                const lamq_ns_f16x8 q = *(lamq_ns_lds_f16x8*)(uintptr_t)(xb + ns_xat(32 * tj + li, 2 * ks + half));
+                T = __builtin_amdgcn_mfma_f32_32x32x16_f16(q, p, T, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                lamq_ns_f16x4 h;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[e] = (_Float16)(T[4 * r + e] * NS_UNSCALE);
+                *at(r) = h;
+            }
+        }
+        __syncthreads();
+        if (mine) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) T[v] = 0.0f;
+#pragma unroll 2
+            for (int ks = 0; ks < 2 * mt; ++ks) {
+                const lamq_ns_f16x8 p = *(lamq_ns_lds_f16x8*)(uintptr_t)(ab + ns_aat(32 * ti + li, 2 * ks + half));
+                const lamq_ns_f16x8 q = *(lamq_ns_lds_f16x8*)(uintptr_t)(ab + ns_aat(32 * tj + li, 2 * ks + half));
+                T = __builtin_amdgcn_mfma_f32_32x32x16_f16(q, p, T, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const lamq_ns_f16x4 h = *at(r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) T[4 * r + e] = fmaf(b, (float)h[e], c * (T[4 * r + e] * NS_UNSCALE));
+            }
+        }
+        __syncthreads();  // A is read
+        if (mine)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                lamq_ns_f16x4 h;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) h[e] = (_Float16)T[4 * r + e];
+                *at(r) = h;
+            }
+        __syncthreads();
+        if (cols) {  // X = a X + B X, onto 2^10 a X
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) X[i][v] *= a * NS_SCALE;
+            for (int ks = 0; ks < 2 * mt; ++ks) {
+                // depth 16 ks + 8 half + {0..7} of a column: two transposing reads of four rows each
+                const int row = 16 * ks + 8 * half + (i16 >> 2), chunk = 4 * wave + 2 * (li >> 4) + ((i16 & 3) >> 1);
+                const lamq_ns_s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lamq_ns_lds_s4*)(uintptr_t)(xb + ns_xat(row, chunk) + 8 * (i16 & 1)));
+                const lamq_ns_s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lamq_ns_lds_s4*)(uintptr_t)(xb + ns_xat(row + 4, chunk) + 8 * (i16 & 1)));
+                const short __attribute__((ext_vector_type(8))) y = __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
+                const lamq_ns_f16x8 q = __builtin_bit_cast(lamq_ns_f16x8, y);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < mt) {
+                        const lamq_ns_f16x8 p = *(lamq_ns_lds_f16x8*)(uintptr_t)(ab + ns_aat(32 * i + li, 2 * ks + half));
+                        X[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q, p, X[i], 0, 0, 0);
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) X[i][v] *= NS_UNSCALE;
+        }
+        __syncthreads();  // X and B are read
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 32 * i + li, col = c0 + 8 * r;
+            uint16_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = __builtin_bit_cast(uint16_t, (__bf16)(X[i][4 * r + e] * NS_UNSCALE));
+            if (!ENTRIES && row < m && col + 4 <= n) {
+                const lamq_ns_u2 w = {(uint32_t)y[0] | ((uint32_t)y[1] << 16), (uint32_t)y[2] | ((uint32_t)y[3] << 16)};
+                *reinterpret_cast<lamq_ns_u2*>(out + row * ldo + col) = w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (row < m && col + e < n) out[tall ? (col + e) * ldo + row : row * ldo + col + e] = y[e];
+            }
+        }
+}
+
 // G as bf16: the result of no step at all
 template <typename Elt>
 __global__ __launch_bounds__(256) void ns_copy_kernel(const Elt* __restrict__ G, int64_t rows, int64_t cols, int64_t ld,
@@ -496,6 +724,13 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
     if (p.mp * p.np > ((int64_t)1 << 36)) return LAMQ_EUNSUP;
     if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < p.total) return LAMQ_EINVAL;
     hipStream_t st = as_stream(stream);
+    const bool tall = rows > cols;
+    if (p.m <= NS_SMALL_M && p.n <= NS_SMALL_N && steps > 0) {
+        hipLaunchKernelGGL((tall || p.n < 4 ? ns_small_kernel<Elt, true> : ns_small_kernel<Elt, false>), dim3((unsigned)batch), dim3(1024), 0, st, G, ld, stride, out, ldo, so, (int)p.m,
+                           (int)p.n, (int)tall, steps, a, b, c);
+        LAMQ_LAUNCH_CHECK();
+        return LAMQ_OK;
+    }
     double* parts = reinterpret_cast<double*>(workspace);
     uint8_t* at = reinterpret_cast<uint8_t*>(parts + batch * NS_PARTS);
     uint16_t* hi[2] = {reinterpret_cast<uint16_t*>(at), reinterpret_cast<uint16_t*>(at + p.x)};
@@ -506,7 +741,6 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
     const int nparts = (int)(want < NS_PARTS ? want : NS_PARTS);
     hipLaunchKernelGGL(ns_norm_kernel<Elt>, dim3(nparts, (unsigned)batch), dim3(256), 0, st, G, rows, cols, ld, stride, parts);
     LAMQ_LAUNCH_CHECK();
-    const bool tall = rows > cols;
     if (steps == 0) {
         hipLaunchKernelGGL(ns_copy_kernel<Elt>, dim3(nparts, (unsigned)batch), dim3(256), 0, st, G, rows, cols, ld, stride,
                            parts, nparts, out, ldo, so);
@@ -537,9 +771,11 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
     x.n = (int)p.n;
     x.tall = tall;
     const dim3 lower((unsigned)(tm * (tm + 1) / 2), (unsigned)batch);
-    // a ring of four stages (all of a unit's LDS) where every tile has a unit to itself, two where two tiles share one;
-    // updates of more tiles than units by tiles of 256 rows: UPDATE_NOTE
-    const bool alone = (int64_t)lower.x * batch <= NS_CUS, wide = (int64_t)tm * tn * batch > NS_CUS;
+    // a ring of four stages (all of a unit's LDS) where every tile has a unit to itself, two where two tiles share one.
+    // Updates take tiles of 256 rows, a third less of X and B through LDS, where two rounds of them fill the chip (9,728 x
+    // 2,560, 760 tiles: 134 us, of 128 rows 137; 2 x 1,024 x 2,560, 160 tiles: 21.9 us, of 128 rows 19.6)
+    const int64_t tiles = (int64_t)tm * tn * batch, tall_tiles = (int64_t)((tm + 1) / 2) * tn * batch;
+    const bool alone = (int64_t)lower.x * batch <= NS_CUS, wide = tall_tiles >= 2 * NS_CUS, apart = tiles <= NS_CUS;
     x.tiles_m = wide ? (tm + 1) / 2 : tm;
     const dim3 full((unsigned)(x.tiles_m * tn), (unsigned)batch), wg(512);
     for (int k = 0; k < steps; ++k) {
@@ -564,10 +800,10 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
         y.sq = p.mp * p.lx;
         y.out = hi[1 - (k & 1)];
         if (k + 1 < steps)
-            hipLaunchKernelGGL((wide ? ns_product_kernel<NS_UPDATE, 4, 3> : ns_product_kernel<NS_UPDATE, 2, 4>), full, wg, 0,
+            hipLaunchKernelGGL((wide ? ns_product_kernel<NS_UPDATE, 4, 3> : apart ? ns_product_kernel<NS_UPDATE, 2, 4> : ns_product_kernel<NS_UPDATE, 2, 2>), full, wg, 0,
                                st, y);
         else
-            hipLaunchKernelGGL((wide ? ns_product_kernel<NS_LAST, 4, 3> : ns_product_kernel<NS_LAST, 2, 4>), full, wg, 0, st,
+            hipLaunchKernelGGL((wide ? ns_product_kernel<NS_LAST, 4, 3> : apart ? ns_product_kernel<NS_LAST, 2, 4> : ns_product_kernel<NS_LAST, 2, 2>), full, wg, 0, st,
                                y);
         LAMQ_LAUNCH_CHECK();
     }

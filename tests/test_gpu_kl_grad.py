@@ -32,7 +32,8 @@ def reference(ref, q, w=None):
     s = torch.where((w != 0)[:, None], s, 0.0)
     lp, ls = torch.log_softmax(r, -1), torch.log_softmax(s, -1)
     p, t = lp.exp(), ls.exp()
-    term = torch.where(lp == -math.inf, 0.0, p * (lp - ls))
+    # a word finite in the reference and -inf in the student makes kl infinite, also where its probability underflows
+    term = torch.where(lp == -math.inf, 0.0, torch.where(ls == -math.inf, math.inf, p * (lp - ls)))
     kl = torch.where(w != 0, term.sum(-1), 0.0)
     coef = torch.where(w != 0, w / w.sum(), 0.0)[:, None]
     grad = coef * (t - p)

@@ -280,43 +280,48 @@ __device__ __forceinline__ void kg_zero(Elt* g, int64_t v0, int64_t v1)
 }
 
 // the workgroup's sum of x, in every thread, in a fixed order
+template <int NT>
 __device__ __forceinline__ double kg_sum(double x)
 {
-    __shared__ double s[KG_NT / 64];
+    __shared__ double s[NT / 64];
     for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
     __syncthreads();
     double t = 0.0;
-    for (int w = 0; w < KG_NT / 64; ++w) t += s[w];
+    for (int w = 0; w < NT / 64; ++w) t += s[w];
     __syncthreads();
     return t;
 }
 
 // sum w (T without weights) over all T, in every thread
+template <int NT>
 __device__ __forceinline__ double kg_weights(const float* __restrict__ w, int64_t T)
 {
     if (!w) return (double)T;
     double x = 0.0;
-    for (int64_t t = threadIdx.x; t < T; t += KG_NT) x += (double)w[t];
-    return kg_sum(x);
+    for (int64_t t = threadIdx.x; t < T; t += NT) x += (double)w[t];
+    return kg_sum<NT>(x);
 }
 
-__global__ __launch_bounds__(KG_NT) void kl_weights_kernel(const float* __restrict__ w, int64_t T,
-                                                           double* __restrict__ total)
+__global__ __launch_bounds__(1024) void kl_weights_kernel(const float* __restrict__ w, int64_t T, double* __restrict__ total)
 {
-    const double x = kg_weights(w, T);
+    const double x = kg_weights<1024>(w, T);
     if (threadIdx.x == 0) *total = x;
 }
 
-// loss = sum w kl / total, of float64 kl's
-__global__ __launch_bounds__(KG_NT) void kl_loss_kernel(const double* __restrict__ kl, const float* __restrict__ w,
-                                                        int64_t T, const double* __restrict__ total,
-                                                        float* __restrict__ loss)
+// loss = sum w kl / sum w, of float64 kl's
+__global__ __launch_bounds__(1024) void kl_loss_kernel(const double* __restrict__ kl, const float* __restrict__ w, int64_t T,
+                                                       float* __restrict__ loss)
 {
-    double x = 0.0;
-    for (int64_t t = threadIdx.x; t < T; t += KG_NT) x += (w ? (double)w[t] : 1.0) * kl[t];
-    x = kg_sum(x);
-    if (threadIdx.x == 0) *loss = (float)(x / *total);
+    double x = 0.0, y = 0.0;
+    for (int64_t t = threadIdx.x; t < T; t += 1024) {
+        const double wt = w ? (double)w[t] : 1.0;
+        x += wt * kl[t];
+        y += wt;
+    }
+    x = kg_sum<1024>(x);
+    y = kg_sum<1024>(y);
+    if (threadIdx.x == 0) *loss = (float)(x / y);
 }
 
 // Many rows: a workgroup of NT threads a row, read once: of a thread's chunks the first REGS stay in its registers and the
@@ -454,7 +459,7 @@ __global__ __launch_bounds__(KG_NT) void kl_grad_part_kernel(const Elt* __restri
         KGPart p{-kg_inf(), -kg_inf(), 0.0, 0.0, 0.0};
         if ((int)threadIdx.x < split) p = parts[t * split + threadIdx.x];
         p = kg_reduce(p);
-        kg_grad(ref + t * ldr, q + t * ldq, grad + t * ldg, v0, v1, kg_coef(p, wt / kg_weights(w, T)));
+        kg_grad(ref + t * ldr, q + t * ldq, grad + t * ldg, v0, v1, kg_coef(p, wt / kg_weights<KG_NT>(w, T)));
         x = kg_kl(p);
     }
     if (s == 0 && threadIdx.x == 0) {
@@ -494,9 +499,9 @@ static int kl_grad_launch(const Elt* ref, const Elt* q, int64_t T, int64_t V, in
     double* kl64 = total + 2;
     KGPart* parts = reinterpret_cast<KGPart*>(kl64 + T);
     const int split = kg_splits(T, V);
-    hipLaunchKernelGGL(kl_weights_kernel, dim3(1), dim3(KG_NT), 0, st, w, T, total);
-    LAMQ_LAUNCH_CHECK();
     if (split == 1) {
+        hipLaunchKernelGGL(kl_weights_kernel, dim3(1), dim3(1024), 0, st, w, T, total);
+        LAMQ_LAUNCH_CHECK();
         // 256 threads hold a row of 16 KB in registers; longer ones take 1,024 threads and most of a unit's LDS
         constexpr int R = sizeof(Elt) == 2 ? 4 : 2;
         if (V <= 8 * 256 * R)
@@ -515,7 +520,7 @@ static int kl_grad_launch(const Elt* ref, const Elt* q, int64_t T, int64_t V, in
                            parts, kl, kl64, grad, ldg);
         LAMQ_LAUNCH_CHECK();
     }
-    hipLaunchKernelGGL(kl_loss_kernel, dim3(1), dim3(KG_NT), 0, st, kl64, w, T, total, loss);
+    hipLaunchKernelGGL(kl_loss_kernel, dim3(1), dim3(1024), 0, st, kl64, w, T, loss);
     LAMQ_LAUNCH_CHECK();
     return LAMQ_OK;
 }

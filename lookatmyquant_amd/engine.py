@@ -643,14 +643,24 @@ def attention_causal(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     return out
 
 
-def _heads(t: torch.Tensor) -> int:
-    """t [B, heads, T, D] as a lamq_heads argument (an address ctypes keeps alive for the call)."""
-    return ctypes.byref(_abi.Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)))
+_HEADS_BYTES = ctypes.sizeof(_abi.Heads)
+
+
+def _heads(*tensors) -> tuple:
+    """[B, heads, T, D] tensors as lamq_heads arguments: the array that holds them (to be kept until the call is over)
+    and each one's address."""
+    flat = []
+    for t in tensors:
+        s = t.stride()
+        flat += (t.data_ptr(), s[0], s[1], s[2])
+    held = (ctypes.c_int64 * len(flat))(*flat)
+    at = ctypes.addressof(held)
+    return held, [at + _HEADS_BYTES * i for i in range(len(tensors))]
 
 
 def _need_heads(t, shape, name: str):
     need(t, torch.bfloat16, name, 4)
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}")
 
 
@@ -659,22 +669,26 @@ def _attention_shapes(q, k, v, lens):
     need(k, torch.bfloat16, "k", 4)
     B, H, T, D = q.shape
     Hkv = k.shape[1]
-    if H < 1 or Hkv < 1 or H % Hkv or tuple(k.shape) != (B, Hkv, T, D):
+    if H < 1 or Hkv < 1 or H % Hkv or k.shape != (B, Hkv, T, D):
         raise ValueError("k and v must be [B, Hkv, T, D] with Hkv dividing q's heads")
     _need_heads(v, k.shape, "v")
     if lens is not None:
         need(lens, torch.int32, "lens", 1)
         if lens.numel() != B:
             raise ValueError("one length per sequence")
-    devs = {t.device for t in (q, k, v) + (() if lens is None else (lens,))}
-    if len(devs) != 1:
-        raise ValueError("all tensors must be on one device")
+    _one_device(q.device, k, v, lens)
     return B, H, Hkv, T, D
+
+
+def _one_device(dev, *tensors):
+    if any(t is not None and t.device != dev for t in tensors):
+        raise ValueError("all tensors must be on one device")
 
 
 def _by_token(B: int, heads: int, T: int, like: torch.Tensor) -> torch.Tensor:
     """An empty [B, heads, T, D] tensor in the layers' [B, T, heads, D] layout."""
-    return torch.empty(B, T, heads, like.shape[3], dtype=like.dtype, device=like.device).transpose(1, 2)
+    D = like.shape[3]
+    return torch.empty_strided((B, heads, T, D), (T * heads * D, D, heads * D, 1), dtype=like.dtype, device=like.device)
 
 
 def attention_causal_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
@@ -684,12 +698,13 @@ def attention_causal_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scal
     scores, which attention_causal_grad takes. Returns (out [B, H, T, 128] bf16, a view of a [B, T, H, 128] buffer,
     lse [B, H, T] float32); tokens past a length have out 0 and lse -inf, and nothing is read there."""
     B, H, Hkv, T, D = _attention_shapes(q, k, v, lens)
+    scale = float(scale)
     out = _by_token(B, H, T, q)
     lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device)
     if B and T:
-        check(lib().lamq_attention_causal_lse_bf16(_heads(q), _heads(k), _heads(v), _heads(out), ptr(lse), ptr(lens), B,
-                                                   H, Hkv, T, D, float(scale), stream(q.device)),
-              "attention_causal_lse")
+        held, at = _heads(q, k, v, out)
+        check(lib().lamq_attention_causal_lse_bf16(*at, lse.data_ptr(), ptr(lens), B, H, Hkv, T, D, scale,
+                                                   stream(q.device)), "attention_causal_lse")
     return out, lse
 
 
@@ -702,17 +717,17 @@ def attention_causal_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, 
     _need_heads(dout, q.shape, "dout")
     _need_heads(out, q.shape, "out")
     need(lse, torch.float32, "lse", 3)
-    if tuple(lse.shape) != (B, H, T) or not lse.is_contiguous():
+    if lse.shape != (B, H, T) or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous [B, H, T]")
-    if {dout.device, out.device, lse.device} != {q.device}:
-        raise ValueError("all tensors must be on one device")
+    _one_device(q.device, dout, out, lse)
+    scale = float(scale)
     dq, dk, dv = _by_token(B, H, T, q), _by_token(B, Hkv, T, q), _by_token(B, Hkv, T, q)
     if B and T:
         nbytes = lib().lamq_attention_causal_grad_workspace_size(B, H, Hkv, T)
         ws = workspace(nbytes, q.device)
-        check(lib().lamq_attention_causal_grad_bf16(_heads(q), _heads(k), _heads(v), _heads(out), ptr(lse),
-                                                    _heads(dout), ptr(lens), _heads(dq), _heads(dk), _heads(dv), B, H,
-                                                    Hkv, T, D, float(scale), ptr(ws), nbytes, stream(q.device)),
+        held, at = _heads(q, k, v, out, dout, dq, dk, dv)
+        check(lib().lamq_attention_causal_grad_bf16(*at[:4], lse.data_ptr(), at[4], ptr(lens), *at[5:], B, H, Hkv, T, D,
+                                                    scale, ws.data_ptr(), nbytes, stream(q.device)),
               "attention_causal_grad")
     return dq, dk, dv
 
@@ -1169,8 +1184,9 @@ def kl_rows_grad(ref: torch.Tensor, q: torch.Tensor, w: torch.Tensor | None = No
     if out is None:
         out = torch.empty(T, V, dtype=dt, device=ref.device)
     need(out, dt, "out", 2)
-    if out.shape != ref.shape or len({ref.device, q.device, out.device}) != 1:
-        raise ValueError("out must be [T, V], all tensors on one device")
+    if out.shape != ref.shape:
+        raise ValueError("out must be [T, V]")
+    _one_device(ref.device, q, out)
     kl = torch.empty(T, dtype=torch.float32, device=ref.device)
     if T == 0:
         return kl, torch.full((), float("nan"), device=ref.device), out

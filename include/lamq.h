@@ -479,6 +479,9 @@ int lamq_attention_causal_bf16(const uint16_t* q, int64_t sqb, int64_t sqh, int6
  *   strides in elements (lamq_heads), the head dim contiguous; strides multiples of 8, inputs 16-byte aligned, what
  *   is written 8-byte aligned and none of it overlapping another tensor.
  *   lse   [B, H, T] float32, written by the forward, read by the backward
+ *   rest  B H ceil(T / 32) 4,096 bf16 bits, 16-byte aligned, or NULL: what out's rounding to bf16 left of it, in the
+ *         kernels' own order, from the forward to the backward's delta (blocks of 32 queries past a length are not
+ *         touched)
  *   lens  [B] int32 on the device, or NULL (all T): tokens past lens[b] (held to 0 .. T) are padding. Nothing is
  *         read there; their rows of out and of the gradients are zeros, their lse -inf.
  * Sums, scores and dP are float32; P and dS are rounded to bf16 as operands of the next product, each result once.
@@ -490,11 +493,11 @@ typedef struct {
     int64_t sb, sh, st;
 } lamq_heads;
 int lamq_attention_causal_lse_bf16(const lamq_heads* q, const lamq_heads* k, const lamq_heads* v, const lamq_heads* out,
-                                   float* lse, const int32_t* lens, int64_t B, int64_t H, int64_t Hkv, int64_t T,
+                                   uint16_t* rest, float* lse, const int32_t* lens, int64_t B, int64_t H, int64_t Hkv, int64_t T,
                                    int64_t D, float scale, void* stream);
 size_t lamq_attention_causal_grad_workspace_size(int64_t B, int64_t H, int64_t Hkv, int64_t T);
 int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_heads* k, const lamq_heads* v, const lamq_heads* out,
-                                    const float* lse, const lamq_heads* dout, const int32_t* lens, const lamq_heads* dq,
+                                    const uint16_t* rest, const float* lse, const lamq_heads* dout, const int32_t* lens, const lamq_heads* dq,
                                     const lamq_heads* dk, const lamq_heads* dv, int64_t B, int64_t H, int64_t Hkv,
                                     int64_t T, int64_t D, float scale, void* workspace, size_t workspace_bytes,
                                     void* stream);

@@ -78,9 +78,9 @@ SIGNATURES = {
                                          _c_flt, _p]),
     "lamq_attention_causal_bf16": (_c_int, [_p] + [_c_i64] * 3 + [_p] + [_c_i64] * 3 + [_p] + [_c_i64] * 3 + [_p]
                                    + [_c_i64] * 3 + [_c_i64] * 5 + [_c_flt, _p]),
-    "lamq_attention_causal_lse_bf16": (_c_int, [_p] * 6 + [_c_i64] * 5 + [_c_flt, _p]),
+    "lamq_attention_causal_lse_bf16": (_c_int, [_p] * 7 + [_c_i64] * 5 + [_c_flt, _p]),
     "lamq_attention_causal_grad_workspace_size": (_c_size, [_c_i64] * 4),
-    "lamq_attention_causal_grad_bf16": (_c_int, [_p] * 10 + [_c_i64] * 5 + [_c_flt, _p, _c_size, _p]),
+    "lamq_attention_causal_grad_bf16": (_c_int, [_p] * 11 + [_c_i64] * 5 + [_c_flt, _p, _c_size, _p]),
     "lamq_orthogonalize_workspace_size": (_c_size, [_c_i64] * 3),
     "lamq_orthogonalize_bf16": (_c_int, [_p] + [_c_i64] * 5 + [_c_int] + [_c_flt] * 3 + [_p, _c_i64, _c_i64, _p, _c_size, _p]),
     "lamq_orthogonalize_f32": (_c_int, [_p] + [_c_i64] * 5 + [_c_int] + [_c_flt] * 3 + [_p, _c_i64, _c_i64, _p, _c_size, _p]),

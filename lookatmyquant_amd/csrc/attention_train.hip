@@ -22,7 +22,10 @@
 // slots, and so do the four rows and four chunks a transposing read serves at once.
 //
 // P is rounded to bf16 for dV as the forward rounds it for O, dS to bf16 for dQ and dK, the operand type of the matrix
-// instructions; scores, dP, delta and every sum are float32, each gradient rounded once at its end.
+// instructions; scores, dP, delta and every sum are float32, each gradient rounded once at its end. delta is a sum of
+// products with O, and where dP - delta is small beside either, O's own rounding would show in dQ and dK (two or three
+// times the rounding of the result, over sequences of a few tokens): the forward leaves what the rounding took, a second
+// bf16 part, for it.
 #include "common.h"
 
 typedef __bf16 lamq_at_bf16x8 __attribute__((ext_vector_type(8)));
@@ -158,22 +161,33 @@ __device__ __forceinline__ void ag_settle(lamq_at_bf16x8 (&f)[8])
     asm volatile("" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]), "+v"(f[4]), "+v"(f[5]), "+v"(f[6]), "+v"(f[7]));
 }
 
+// O's second part is kept by blocks of 32 queries, [16 chunks of 8 head dims][32 queries][8]: the writer's 8 bytes a lane
+// and the reader's 16 are 512 bytes in a row a load or store. The offset of a query's first chunk.
+__device__ __forceinline__ int64_t ag_rest(int head, int T, int q0, int li)
+{
+    return ((int64_t)head * ((T + 31) / 32) + q0 / 32) * (32 * AT_D) + 8 * li;
+}
+
 // a transposed 128 x 32 result (four tiles: head dims 32 t + 8 r + 4 hi + {0..3} of the lane's row) times `scale`, as
-// bf16 (nearest, ties to even) into the row
-__device__ __forceinline__ void ag_store_row(uint16_t* row, const lamq_at_f32x16 (&acc)[4], float scale, int hi)
+// bf16 (nearest, ties to even) into the row; what the rounding leaves of it, as bf16 again, into `rest` if there is one
+__device__ __forceinline__ void ag_store_row(uint16_t* row, const lamq_at_f32x16 (&acc)[4], float scale, int hi,
+                                             uint16_t* rest = nullptr)
 {
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            uint32_t w2[2];
+            uint32_t w2[2], l2[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const __bf16 x0 = (__bf16)(acc[t][4 * r + 2 * e] * scale);
-                const __bf16 x1 = (__bf16)(acc[t][4 * r + 2 * e + 1] * scale);
+                const float f0 = acc[t][4 * r + 2 * e] * scale, f1 = acc[t][4 * r + 2 * e + 1] * scale;
+                const __bf16 x0 = (__bf16)f0, x1 = (__bf16)f1;
+                const __bf16 y0 = (__bf16)(f0 - (float)x0), y1 = (__bf16)(f1 - (float)x1);
                 w2[e] = (uint32_t)__builtin_bit_cast(uint16_t, x0) | ((uint32_t)__builtin_bit_cast(uint16_t, x1) << 16);
+                l2[e] = (uint32_t)__builtin_bit_cast(uint16_t, y0) | ((uint32_t)__builtin_bit_cast(uint16_t, y1) << 16);
             }
             *reinterpret_cast<uint2*>(row + 32 * t + 8 * r + 4 * hi) = make_uint2(w2[0], w2[1]);
+            if (rest) *reinterpret_cast<uint2*>(rest + (4 * t + r) * 256) = make_uint2(l2[0], l2[1]);
         }
 }
 
@@ -201,8 +215,8 @@ __device__ __forceinline__ bool ag_place(int pairs, int per, int& pair, int& rem
 // The sums of a query's two lanes are added at the end. 4 x 32 heads x 2,048: 195 -> FWD us against the exact maximum and
 // 32 keys a step.
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_lse_kernel(
-    AtView Q, AtView K, AtView V, AtOut O, float* __restrict__ lse, const int32_t* __restrict__ lens, int rep, int Hkv,
-    int pairs, int Tall, float scale_log2)
+    AtView Q, AtView K, AtView V, AtOut O, uint16_t* __restrict__ rest, float* __restrict__ lse,
+    const int32_t* __restrict__ lens, int rep, int Hkv, int pairs, int Tall, float scale_log2)
 {
     __shared__ __align__(256) uint8_t lds[2][2][AG_OPB];  // [buffer][K, V]
     const int nqb = (Tall + AG_OWN - 1) / AG_OWN;
@@ -313,14 +327,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
     if (myq >= T) return;
     sum = at_sum32(sum);
-    ag_store_row(Op + (int64_t)myq * O.st, o, 1.0f / sum, hi);
+    ag_store_row(Op + (int64_t)myq * O.st, o, 1.0f / sum, hi,
+                 rest ? rest + ag_rest(b * Hkv * rep + h, Tall, q0, li) + 4 * hi : nullptr);
     if (hi == 0) L[myq] = (m + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
 }
 
 // dQ, and per query the log-sum-exp in units of log 2 and delta for the other kernel (rows [B, H, T] of stats and
 // stats + B H T).
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_dq_kernel(
-    AtView Q, AtView K, AtView V, AtView O, AtView dO, AtOut dQ, const float* __restrict__ lse,
+    AtView Q, AtView K, AtView V, AtView O, AtView dO, AtOut dQ, const uint16_t* __restrict__ rest,
+    const float* __restrict__ lse,
     const int32_t* __restrict__ lens, float* __restrict__ stats, int64_t nstats, int rep, int Hkv, int pairs, int Tall,
     float scale, float scale_log2)
 {
@@ -359,20 +375,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         const uint16_t* Qr = Q.p + b * Q.sb + (int64_t)h * Q.sh + (int64_t)qrow * Q.st + 8 * hi;
         const uint16_t* Dr = dO.p + b * dO.sb + (int64_t)h * dO.sh + (int64_t)qrow * dO.st + 8 * hi;
         const uint16_t* Or = O.p + b * O.sb + (int64_t)h * O.sh + (int64_t)qrow * O.st + 8 * hi;
-        lamq_at_bf16x8 of[8];
+        const uint16_t* Lr = rest + ag_rest(b * Hkv * rep + h, Tall, q0, li) + 256 * hi;
+        const int64_t at = ((int64_t)b * Hkv * rep + h) * Tall + qrow;
+        lse2 = lse[at] * AT_LOG2E;
+        lamq_at_bf16x8 of[8], lf[8];
+        // O's second part has blocks only up to T, and rows only up to the length
+        const bool second = rest && myq < T;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             qf[j] = ag_row8(Qr + 16 * j);
             df[j] = ag_row8(Dr + 16 * j);
             of[j] = ag_row8(Or + 16 * j);
+            lf[j] = of[j];
         }
+        if (second)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) lf[j] = ag_row8(Lr + 512 * j);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = fmaf((float)df[j][e], (float)of[j][e], delta);
+        if (second)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) delta = fmaf((float)df[j][e], (float)lf[j][e], delta);
         delta = at_sum32(delta);
-        const int64_t at = ((int64_t)b * Hkv * rep + h) * Tall + qrow;
-        lse2 = lse[at] * AT_LOG2E;
         if (hi == 0 && myq < T) {
             stats[at] = lse2;
             stats[nstats + at] = delta;
@@ -603,18 +631,19 @@ static AtView at_view(const lamq_heads* x) { return AtView{x->data, x->sb, x->sh
 static AtOut at_out(const lamq_heads* x) { return AtOut{x->data, x->sb, x->sh, x->st}; }
 
 extern "C" int lamq_attention_causal_lse_bf16(const lamq_heads* q, const lamq_heads* k, const lamq_heads* v,
-                                              const lamq_heads* out, float* lse, const int32_t* lens, int64_t B,
-                                              int64_t H, int64_t Hkv, int64_t T, int64_t D, float scale, void* stream)
+                                              const lamq_heads* out, uint16_t* rest, float* lse, const int32_t* lens,
+                                              int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t D, float scale,
+                                              void* stream)
 {
     int rc = at_sizes(B, H, Hkv, T, D, scale);
     for (const lamq_heads* x : {q, k, v})
         if (rc == LAMQ_OK) rc = at_heads(x, T, 16);
     if (rc == LAMQ_OK) rc = at_heads(out, T, 8);
     if (rc != LAMQ_OK) return rc;
-    if (!lse) return LAMQ_EINVAL;
+    if (!lse || (uintptr_t)rest % 16) return LAMQ_EINVAL;
     if (B == 0 || T == 0) return LAMQ_OK;
     hipLaunchKernelGGL(attention_lse_kernel, at_grid(cdiv(T, AG_OWN) * H * B), dim3(256), 0, as_stream(stream), at_view(q),
-                       at_view(k), at_view(v), at_out(out), lse, lens, (int)(H / Hkv), (int)Hkv, (int)(B * Hkv), (int)T,
+                       at_view(k), at_view(v), at_out(out), rest, lse, lens, (int)(H / Hkv), (int)Hkv, (int)(B * Hkv), (int)T,
                        scale * AT_LOG2E);
     LAMQ_LAUNCH_CHECK();
     return LAMQ_OK;
@@ -627,7 +656,8 @@ extern "C" size_t lamq_attention_causal_grad_workspace_size(int64_t B, int64_t H
 }
 
 extern "C" int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_heads* k, const lamq_heads* v,
-                                               const lamq_heads* out, const float* lse, const lamq_heads* dout,
+                                               const lamq_heads* out, const uint16_t* rest, const float* lse,
+                                               const lamq_heads* dout,
                                                const int32_t* lens, const lamq_heads* dq, const lamq_heads* dk,
                                                const lamq_heads* dv, int64_t B, int64_t H, int64_t Hkv, int64_t T,
                                                int64_t D, float scale, void* workspace, size_t workspace_bytes,
@@ -639,7 +669,7 @@ extern "C" int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_h
     for (const lamq_heads* x : {dq, dk, dv})
         if (rc == LAMQ_OK) rc = at_heads(x, T, 8);
     if (rc != LAMQ_OK) return rc;
-    if (!lse) return LAMQ_EINVAL;
+    if (!lse || (uintptr_t)rest % 16) return LAMQ_EINVAL;
     if (B == 0 || T == 0) return LAMQ_OK;
     if (!workspace || (uintptr_t)workspace % 4 ||
         workspace_bytes < lamq_attention_causal_grad_workspace_size(B, H, Hkv, T))
@@ -648,7 +678,7 @@ extern "C" int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_h
     const int64_t nstats = B * H * T;
     hipStream_t s = as_stream(stream);
     hipLaunchKernelGGL(attention_dq_kernel, at_grid(cdiv(T, AG_OWN) * H * B), dim3(256), 0, s, at_view(q), at_view(k),
-                       at_view(v), at_view(out), at_view(dout), at_out(dq), lse, lens, stats, nstats, (int)(H / Hkv),
+                       at_view(v), at_view(out), at_view(dout), at_out(dq), rest, lse, lens, stats, nstats, (int)(H / Hkv),
                        (int)Hkv, (int)(B * Hkv), (int)T, scale, scale * AT_LOG2E);
     LAMQ_LAUNCH_CHECK();
     hipLaunchKernelGGL(attention_dkdv_kernel, at_grid(cdiv(T, AG_KEYS) * Hkv * B), dim3(256), 0, s, at_view(q), at_view(k),

@@ -565,7 +565,6 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
         if (mine) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) T[v] = 0.0f;
-#pragma unroll 2
             for (int ks = 0; ks < 2 * nt; ++ks) {
                 const lamq_ns_f16x8 p = *(lamq_ns_lds_f16x8*)(uintptr_t)(xb + ns_xat(32 * ti + li, 2 * ks + half));
                 const lamq_ns_f16x8 q = *(lamq_ns_lds_f16x8*)(uintptr_t)(xb + ns_xat(32 * tj + li, 2 * ks + half));
@@ -583,7 +582,6 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
         if (mine) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) T[v] = 0.0f;
-#pragma unroll 2
             for (int ks = 0; ks < 2 * mt; ++ks) {
                 const lamq_ns_f16x8 p = *(lamq_ns_lds_f16x8*)(uintptr_t)(ab + ns_aat(32 * ti + li, 2 * ks + half));
                 const lamq_ns_f16x8 q = *(lamq_ns_lds_f16x8*)(uintptr_t)(ab + ns_aat(32 * tj + li, 2 * ks + half));

@@ -29,17 +29,17 @@ from . import stack
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, lens):
-        out, lse = E.attention_causal_lse(q, k, v, scale, lens)
-        ctx.save_for_backward(q, k, v, out, lse, lens)
+        out, kept = E.attention_causal_lse(q, k, v, scale, lens)
+        ctx.save_for_backward(q, k, v, out, *kept, lens)
         ctx.scale = scale
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, lens = ctx.saved_tensors
+        q, k, v, out, lse, rest, lens = ctx.saved_tensors
         if dout.stride(-1) != 1 or any(s % 8 for s in dout.stride()[:3]) or dout.data_ptr() % 16:
             dout = dout.contiguous()  # e.g. a sum's gradient, one value for all
-        return (*E.attention_causal_grad(dout, q, k, v, out, lse, ctx.scale, lens), None, None)
+        return (*E.attention_causal_grad(dout, q, k, v, out, E.AttentionKept(lse, rest), ctx.scale, lens), None, None)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, lens: torch.Tensor | None = None):

@@ -7,6 +7,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 from functools import lru_cache
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -691,42 +692,58 @@ def _by_token(B: int, heads: int, T: int, like: torch.Tensor) -> torch.Tensor:
     return torch.empty_strided((B, heads, T, D), (T * heads * D, D, heads * D, 1), dtype=like.dtype, device=like.device)
 
 
+class AttentionKept(NamedTuple):
+    """What attention_causal_grad needs of attention_causal_lse beside its out: the log-sum-exp of every query's scaled
+    scores (float32 [B, H, T], -inf past a length), and what out's rounding to bf16 left of it (bf16, in the kernels' own
+    order)."""
+
+    lse: torch.Tensor
+    rest: torch.Tensor
+
+
+def _rest_size(B: int, H: int, T: int) -> int:
+    return B * H * ((T + 31) // 32) * 4096
+
+
 def attention_causal_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float,
-                         lens: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                         lens: torch.Tensor | None = None) -> tuple[torch.Tensor, AttentionKept]:
     """The attention of training (lamq_attention_causal_lse_bf16): attention_causal over the first lens[b] tokens of
-    each sequence (int32 [B] on the device, held to 0 .. T; None: all T), and the log-sum-exp of every query's scaled
-    scores, which attention_causal_grad takes. Returns (out [B, H, T, 128] bf16, a view of a [B, T, H, 128] buffer,
-    lse [B, H, T] float32); tokens past a length have out 0 and lse -inf, and nothing is read there."""
+    each sequence (int32 [B] on the device, held to 0 .. T; None: all T), with what its gradient needs. Returns (out
+    [B, H, T, 128] bf16, in a [B, T, H, 128] layout, AttentionKept); tokens past a length have out 0 and lse -inf, and
+    nothing is read there."""
     B, H, Hkv, T, D = _attention_shapes(q, k, v, lens)
     scale = float(scale)
     out = _by_token(B, H, T, q)
     lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device)
+    rest = torch.empty(_rest_size(B, H, T), dtype=torch.bfloat16, device=q.device)
     if B and T:
         held, at = _heads(q, k, v, out)
-        check(lib().lamq_attention_causal_lse_bf16(*at, lse.data_ptr(), ptr(lens), B, H, Hkv, T, D, scale,
+        check(lib().lamq_attention_causal_lse_bf16(*at, rest.data_ptr(), lse.data_ptr(), ptr(lens), B, H, Hkv, T, D, scale,
                                                    stream(q.device)), "attention_causal_lse")
-    return out, lse
+    return out, AttentionKept(lse, rest)
 
 
 def attention_causal_grad(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
-                          lse: torch.Tensor, scale: float, lens: torch.Tensor | None = None) -> tuple:
+                          kept: AttentionKept, scale: float, lens: torch.Tensor | None = None) -> tuple:
     """The gradients of attention_causal_lse (lamq_attention_causal_grad_bf16) for the gradient dout of its out: (dq
-    [B, H, T, 128], dk, dv [B, Hkv, T, 128]) bf16, views of [B, T, heads, 128] buffers, zero past a length. out and lse
-    are the forward's, scale and lens the ones it was given."""
+    [B, H, T, 128], dk, dv [B, Hkv, T, 128]) bf16, in [B, T, heads, 128] layouts, zero past a length. out and kept are the
+    forward's, scale and lens the ones it was given."""
     B, H, Hkv, T, D = _attention_shapes(q, k, v, lens)
     _need_heads(dout, q.shape, "dout")
     _need_heads(out, q.shape, "out")
+    lse, rest = kept
     need(lse, torch.float32, "lse", 3)
-    if lse.shape != (B, H, T) or not lse.is_contiguous():
-        raise ValueError("lse must be a contiguous [B, H, T]")
-    _one_device(q.device, dout, out, lse)
+    need(rest, torch.bfloat16, "rest", 1)
+    if lse.shape != (B, H, T) or not lse.is_contiguous() or rest.numel() != _rest_size(B, H, T):
+        raise ValueError("lse must be a contiguous [B, H, T], rest the forward's")
+    _one_device(q.device, dout, out, lse, rest)
     scale = float(scale)
     dq, dk, dv = _by_token(B, H, T, q), _by_token(B, Hkv, T, q), _by_token(B, Hkv, T, q)
     if B and T:
         nbytes = lib().lamq_attention_causal_grad_workspace_size(B, H, Hkv, T)
         ws = workspace(nbytes, q.device)
         held, at = _heads(q, k, v, out, dout, dq, dk, dv)
-        check(lib().lamq_attention_causal_grad_bf16(*at[:4], lse.data_ptr(), at[4], ptr(lens), *at[5:], B, H, Hkv, T, D,
+        check(lib().lamq_attention_causal_grad_bf16(*at[:4], rest.data_ptr(), lse.data_ptr(), at[4], ptr(lens), *at[5:], B, H, Hkv, T, D,
                                                     scale, ws.data_ptr(), nbytes, stream(q.device)),
               "attention_causal_grad")
     return dq, dk, dv

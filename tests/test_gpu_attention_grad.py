@@ -57,7 +57,8 @@ def reference(q, k, v, do, scale, lens=None):
     es = 2 * U32 * (D * scale * (q.abs() @ kk.abs().mT) + 4 * s.abs().masked_fill(~seen, 0.0) + 4 * lse.abs().masked_fill(~live, 0.0) + 4)
     ep = p * es.masked_fill(~seen, 0.0)
     eout = (U16 * p + 2 * ep) @ vv.abs() + 2 * T * U32 * (p @ vv.abs()) + U16 * out.abs()
-    edelta = (do.abs() * eout).sum(-1, keepdim=True) + 2 * D * U32 * (do.abs() * out.abs()).sum(-1, keepdim=True)
+    # delta takes O before its rounding, to 2^-16 of it: what is left of O's error are P's roundings
+    edelta = (do.abs() * (eout - (U16 - U16 ** 2) * out.abs())).sum(-1, keepdim=True) + 2 * D * U32 * (do.abs() * out.abs()).sum(-1, keepdim=True)
     edp = 2 * D * U32 * (do.abs() @ vv.abs().mT) + 2 * U32 * delta.abs()
     eds = U16 * ds.abs() + ep * (dp - delta).abs() + p * (edelta + edp)
     sums = 2 * T * rep * U32
@@ -81,10 +82,10 @@ def check(got, want, tol):
 def ours(q, k, v, do, scale, lens=None):
     from lookatmyquant_amd import engine as E
 
-    out, lse = E.attention_causal_lse(q, k, v, scale, lens)
-    dq, dk, dv = E.attention_causal_grad(do, q, k, v, out, lse, scale, lens)
+    out, kept = E.attention_causal_lse(q, k, v, scale, lens)
+    dq, dk, dv = E.attention_causal_grad(do, q, k, v, out, kept, scale, lens)
     torch.cuda.synchronize()
-    return {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
+    return {"out": out, "lse": kept.lse, "dq": dq, "dk": dk, "dv": dv}
 
 
 @pytest.mark.parametrize("B,H,Hkv,T", [(1, 1, 1, 1), (2, 4, 2, 2), (1, 8, 2, 31), (3, 3, 3, 32), (1, 4, 1, 33),
@@ -116,6 +117,21 @@ def test_lengths_and_what_padding_holds(T, lens):
         for nm in ("out", "dq", "dk", "dv"):
             assert bool((got[nm][b, :, max(0, m):] == 0).all()), nm
         assert bool((got["lse"][b, :, max(0, m):] == -math.inf).all())
+
+
+def test_second_part_is_read_where_it_was_written():
+    """Of O's second part only the rows of queries below the length count: what the others hold reaches nothing."""
+    from lookatmyquant_amd import engine as E
+
+    q, k, v, do = inputs(2, 2, 2, 40, 61)
+    lens = torch.tensor([40, 7], dtype=torch.int32, device="cuda")
+    out, kept = E.attention_causal_lse(q, k, v, SCALE, lens)
+    want = E.attention_causal_grad(do, q, k, v, out, kept, SCALE, lens)
+    rows = kept.rest.view(2, 2, 2, 16, 32, 8)  # [sequence, head, block of 32 queries, chunk, query, 8 head dims]
+    assert bool(torch.isfinite(rows[0, :, 0]).all()) and bool(torch.isfinite(rows[0, :, 1, :, :8]).all())
+    rows[0, :, 1, :, 8:], rows[1, :, 0, :, 7:], rows[1, :, 1] = float("nan"), float("nan"), float("nan")
+    got = E.attention_causal_grad(do, q, k, v, out, kept, SCALE, lens)
+    assert all(torch.equal(a, b) and bool(torch.isfinite(a).all()) for a, b in zip(got, want))
 
 
 @pytest.mark.parametrize("gain", [0.0, 0.05, 4.0])
@@ -203,7 +219,8 @@ def test_refusals():
     from lookatmyquant_amd import engine as E
 
     q, k, v, do = inputs(2, 4, 2, 40, 51)
-    out, lse = E.attention_causal_lse(q, k, v, SCALE)
+    out, kept = E.attention_causal_lse(q, k, v, SCALE)
+    lse, rest = kept
     for bad in ((q.float(), k, v), (q, k[:, :, :39], v), (q, k, v[:1]), (q.cpu(), k, v), (q[:, :3], k, v)):
         with pytest.raises(ValueError):
             E.attention_causal_lse(*bad, SCALE)
@@ -219,12 +236,13 @@ def test_refusals():
     odd = torch.empty(2, 40, 4, D + 4, dtype=torch.bfloat16, device="cuda")[..., :D].transpose(1, 2)
     with pytest.raises(ValueError):  # rows that do not start 16-byte aligned
         E.attention_causal_lse(odd, k, v, SCALE)
-    for bad in ((do[:, :, :39], q, k, v, out, lse), (do, q, k, v, out.float(), lse), (do, q, k, v, out, lse[:, :3]),
-                (do, q, k, v, out, lse.double()), (do.transpose(2, 3), q, k, v, out, lse)):
+    for bad in ((do[:, :, :39], q, k, v, out, kept), (do, q, k, v, out.float(), kept), (do, q, k, v, out, (lse[:, :3], rest)),
+                (do, q, k, v, out, (lse.double(), rest)), (do.transpose(2, 3), q, k, v, out, kept),
+                (do, q, k, v, out, (lse, rest[:-1])), (do, q, k, v, out, (lse, rest.float()))):
         with pytest.raises(ValueError):
             E.attention_causal_grad(*bad, SCALE)
     empty = E.attention_causal_lse(q[:0], k[:0], v[:0], SCALE)
-    assert empty[0].shape == (0, 4, 40, D) and empty[1].shape == (0, 4, 40)
+    assert empty[0].shape == (0, 4, 40, D) and empty[1].lse.shape == (0, 4, 40)
     none = E.attention_causal_grad(do[:, :, :0], q[:, :, :0], k[:, :, :0], v[:, :, :0], out[:, :, :0],
-                                   lse[:, :, :0].contiguous(), SCALE)
+                                   (lse[:, :, :0].contiguous(), rest[:0]), SCALE)
     assert none[0].shape == (2, 4, 0, D) and none[1].shape == (2, 2, 0, D)

@@ -121,31 +121,57 @@ __global__ __launch_bounds__(256) void ns_start_kernel(const Elt* __restrict__ G
                                                        int mp, int lx, uint16_t* __restrict__ hi,
                                                        uint16_t* __restrict__ lo)
 {
-    __shared__ float tile[64][65];
     const int64_t batch = blockIdx.z;
     const double ss = ns_sum((int)threadIdx.x < nparts ? parts[batch * nparts + threadIdx.x] : 0.0);
     const double f = ss > 0.0 ? (double)NS_SCALE / sqrt(ss) : ss;  // NaN stays
     const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-    const int x = threadIdx.x & 63;
     const Elt* g = G + batch * stride;
+    if constexpr (!TALL) {  // eight entries of a row a lane
+        const int x = threadIdx.x & 7;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t r = r0 + 32 * h + (threadIdx.x >> 3), c = c0 + 8 * x;
+            float v[8];
+            const int64_t left = cols - c;
+            if (r < rows && left > 0)
+                ns_load8(g + r * ld + c, left < 8 ? (int)left : 8, v);
+            else
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+            lamq_ns_f16x8 hv, lv;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = (float)((double)v[e] * f);
+                hv[e] = (_Float16)y;
+                lv[e] = (_Float16)(y - (float)hv[e]);
+            }
+            const int64_t at = (batch * mp + r) * (int64_t)lx + c;
+            *reinterpret_cast<lamq_ns_f16x8*>(hi + at) = hv;
+            *reinterpret_cast<lamq_ns_f16x8*>(lo + at) = lv;
+        }
+    } else {  // along G's rows into LDS, then eight entries of a row of X a lane
+        __shared__ float tile[64][65];
+        const int x = threadIdx.x & 63;
 #pragma unroll 4
-    for (int y = threadIdx.x >> 6; y < 64; y += 4) {
-        // the tile in G's own order: along its rows
-        const int64_t r = (TALL ? c0 : r0) + y, c = (TALL ? r0 : c0) + x;
-        const float v = r < rows && c < cols ? (float)((double)ns_load(g + r * ld + c) * f) : 0.0f;
-        if (TALL)
-            tile[x][y] = v;
-        else
-            tile[y][x] = v;
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int y = threadIdx.x >> 6; y < 64; y += 4) {
-        const float v = tile[y][x];
-        const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
-        const int64_t at = (batch * mp + r0 + y) * (int64_t)lx + c0 + x;
-        hi[at] = __builtin_bit_cast(uint16_t, h);
-        lo[at] = __builtin_bit_cast(uint16_t, l);
+        for (int y = threadIdx.x >> 6; y < 64; y += 4) {
+            const int64_t r = c0 + y, c = r0 + x;
+            tile[x][y] = r < rows && c < cols ? (float)((double)ns_load(g + r * ld + c) * f) : 0.0f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int y = 32 * h + (threadIdx.x >> 3), c = 8 * (threadIdx.x & 7);
+            lamq_ns_f16x8 hv, lv;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = tile[y][c + e];
+                hv[e] = (_Float16)v;
+                lv[e] = (_Float16)(v - (float)hv[e]);
+            }
+            const int64_t at = (batch * mp + r0 + y) * (int64_t)lx + c0 + c;
+            *reinterpret_cast<lamq_ns_f16x8*>(hi + at) = hv;
+            *reinterpret_cast<lamq_ns_f16x8*>(lo + at) = lv;
+        }
     }
 }
 
@@ -292,6 +318,35 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
             }
         }
     };
+    // What the end of the tile reads, A or X there, is asked for before the products where there are registers for it (a
+    // tile that has a unit to itself, whose end nothing else covers: 1.5 us of a launch)
+    constexpr bool EARLY = RING > 3;
+    static_assert(!EARLY || MT == 2, "the early loads are of one 64-row part of a 128-row tile, always inside X");
+    lamq_ns_f16x4 A[MODE == NS_POLY && EARLY ? 2 * MT * 4 : 1];
+    lamq_ns_f16x8 H[8], L[8];
+    const int r8 = lane >> 3, c8 = lane & 7;
+    auto a_at = [&](int i, int j, int r) {
+        return (batch * g.mp + I * 64 * MT + wm + 32 * i + li) * (int64_t)g.la + J * NS_T + wn + 32 * j + 8 * r + 4 * half;
+    };
+    auto x_at = [&](int h, int y) {
+        return (batch * g.mp + I * 64 * MT + wm + 64 * h + 8 * y + r8) * (int64_t)g.lx + J * NS_T + wn + 8 * c8;
+    };
+    if constexpr (EARLY && MODE == NS_POLY) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    A[8 * i + 4 * j + r] = *reinterpret_cast<const lamq_ns_f16x4*>(g.in_hi + a_at(i, j, r));
+    }
+    if constexpr (EARLY && !SYM) {
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            H[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.in_hi + x_at(0, y));
+            L[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.out_lo + x_at(0, y));
+        }
+    }
     lamq_ns_f16x8 pf[2][MT], qf[2][2];
     for (int st = 0; st < nst; ++st) {
         __syncthreads();  // the stage has landed
@@ -324,14 +379,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int col = J * NS_T + wn + 32 * j + 8 * r + 4 * half;
-                    const int64_t at = (batch * g.mp + row) * (int64_t)g.la + col;
+                    const int64_t at = a_at(i, j, r);
                     float x[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * r + e] * NS_UNSCALE;
                     if (MODE == NS_POLY) {
-                        const lamq_ns_f16x4 A = *reinterpret_cast<const lamq_ns_f16x4*>(g.in_hi + at);
+                        const lamq_ns_f16x4 a =
+                            EARLY ? A[EARLY ? 8 * i + 4 * j + r : 0] : *reinterpret_cast<const lamq_ns_f16x4*>(g.in_hi + at);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = fmaf(g.b, (float)A[e], g.c * x[e]);
+                        for (int e = 0; e < 4; ++e) x[e] = fmaf(g.b, (float)a[e], g.c * x[e]);
                     }
                     lamq_ns_f16x4 o;
 #pragma unroll
@@ -354,13 +410,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
         for (int h = 0; h < MT / 2; ++h) {  // 64 rows at a time
             const int m0 = I * 64 * MT + wm + 64 * h;
             if (m0 >= g.mp) break;  // uniform: past the matrix
-            const int r8 = lane >> 3, c8 = lane & 7;
-            const int64_t at0 = (batch * g.mp + m0 + r8) * (int64_t)g.lx + J * NS_T + wn + 8 * c8;
-            lamq_ns_f16x8 H[8], L[8];
+            if constexpr (!EARLY) {
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                H[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.in_hi + at0 + (int64_t)(8 * y) * g.lx);
-                L[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.lx);
+                for (int y = 0; y < 8; ++y) {
+                    H[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.in_hi + x_at(h, y));
+                    L[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.out_lo + x_at(h, y));
+                }
             }
             float4* tile = reinterpret_cast<float4*>(lds) + wv * 1024;
 #pragma unroll
@@ -389,8 +444,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
                         hv[e] = (_Float16)x[e];
                         lv[e] = (_Float16)(x[e] - (float)hv[e]);
                     }
-                    *reinterpret_cast<lamq_ns_f16x8*>(g.out + at0 + (int64_t)(8 * y) * g.lx) = hv;
-                    *reinterpret_cast<lamq_ns_f16x8*>(g.out_lo + at0 + (int64_t)(8 * y) * g.lx) = lv;
+                    *reinterpret_cast<lamq_ns_f16x8*>(g.out + x_at(h, y)) = hv;
+                    *reinterpret_cast<lamq_ns_f16x8*>(g.out_lo + x_at(h, y)) = lv;
                 } else if (g.tall) {  // back where it was, to be read by columns
                     *t0 = make_float4(x[0], x[1], x[2], x[3]);
                     *t1 = make_float4(x[4], x[5], x[6], x[7]);

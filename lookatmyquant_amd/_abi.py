@@ -148,7 +148,8 @@ def device() -> torch.device:
 
 
 def stream(dev: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    index = torch.cuda.current_device() if dev is None or dev.index is None else dev.index
+    return torch._C._cuda_getCurrentRawStream(index)  # current_stream(dev).cuda_stream without the Stream object
 
 
 def ptr(t: torch.Tensor | None):

@@ -12,6 +12,13 @@
 // below. All sums are float32. X, A and B are stored times 2^10 (exact), which keeps entries of 1e-4, as a normalised
 // large matrix has, clear of float16's smallest normal number; the largest entries, below 8, stay below 2^13.
 //
+// A's and B's entries are largest on the diagonal (near 1 and 2 at the end), and with few rows their rounding to float16
+// there moves a whole singular direction (2e-3 to 4e-3 at 1 to 7 rows, more than the result's own rounding). The
+// diagonals are therefore kept in float32 beside the matrices, and what float16 took of them is put back entry by entry:
+// with A = Ah + E, E diagonal, A^2 = Ah^2 + E A + A E (E^2 is below 2^-24), and with B = Bh + F and X = H + L,
+// B X = Bh H + F H + diag(B) L (L's other products stay out, as everywhere). 1 x 900 to 7 x 659: below 7e-4; 1,001 x 333
+// 3.0e-4 -> 2.0e-4.
+//
 // A and B are symmetric: only the tiles on and below the diagonal are computed and each is stored twice. Sizes are
 // padded with zeros to tiles, which changes no entry of any product.
 #include "common.h"
@@ -34,6 +41,9 @@ typedef __attribute__((address_space(3))) const lamq_ns_f16x8 lamq_ns_lds_f16x8;
 #define NS_PARTS 256                 // partial sums of squares a matrix
 #define NS_SCALE 1024.0f             // what X, A and B are stored times
 #define NS_UNSCALE (1.0f / 1024.0f)
+
+// what float16 takes of a value
+__device__ __forceinline__ float ns_rest(float d) { return d - (float)(_Float16)d; }
 
 __device__ __forceinline__ float ns_load(const float* p) { return *p; }
 __device__ __forceinline__ float ns_load(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
@@ -213,6 +223,8 @@ struct NSArgs {
     int K, tiles_m, mp, lx, la;  // rows of X lx apart, of A and B la
     uint16_t *out, *out_lo;  // A, B or the next X's hi; lo (read and written in place)
     const uint16_t* in_hi;   // poly: A; update: X's hi
+    float* diag;             // gram: A's diagonal, poly: B's, [..][mp]
+    const float* in_diag;    // poly: A's, update: B's
     float a, b, c;
     uint16_t* bf;  // last: the caller's matrix
     int64_t ldb, sb;
@@ -324,6 +336,9 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
     static_assert(!EARLY || MT == 2, "the early loads are of one 64-row part of a 128-row tile, always inside X");
     lamq_ns_f16x4 A[MODE == NS_POLY && EARLY ? 2 * MT * 4 : 1];
     lamq_ns_f16x8 H[8], L[8];
+    float4 dcol[MODE == NS_POLY && EARLY ? 8 : 1];
+    float drow[MODE == NS_POLY && EARLY ? MT : 1], dx = 0.0f;
+    const float* D = g.in_diag + batch * g.mp;
     const int r8 = lane >> 3, c8 = lane & 7;
     auto a_at = [&](int i, int j, int r) {
         return (batch * g.mp + I * 64 * MT + wm + 32 * i + li) * (int64_t)g.la + J * NS_T + wn + 32 * j + 8 * r + 4 * half;
@@ -331,7 +346,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
     auto x_at = [&](int h, int y) {
         return (batch * g.mp + I * 64 * MT + wm + 64 * h + 8 * y + r8) * (int64_t)g.lx + J * NS_T + wn + 8 * c8;
     };
+    auto d_row = [&](int i) { return D[I * 64 * MT + wm + 32 * i + li]; };
+    auto d_col = [&](int j, int r) { return *reinterpret_cast<const float4*>(D + J * NS_T + wn + 32 * j + 8 * r + 4 * half); };
     if constexpr (EARLY && MODE == NS_POLY) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) drow[i] = d_row(i);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dcol[4 * j + r] = d_col(j, r);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -341,6 +364,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
                     A[8 * i + 4 * j + r] = *reinterpret_cast<const lamq_ns_f16x4*>(g.in_hi + a_at(i, j, r));
     }
     if constexpr (EARLY && !SYM) {
+        dx = D[I * 64 * MT + wm + lane];
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
             H[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.in_hi + x_at(0, y));
@@ -374,6 +398,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             const int row = I * 64 * MT + wm + 32 * i + li;
+            const float er = MODE == NS_POLY ? ns_rest(EARLY ? drow[EARLY ? i : 0] : d_row(i)) : 0.0f;
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -382,16 +407,26 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
                     const int64_t at = a_at(i, j, r);
                     float x[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * r + e] * NS_UNSCALE;
+                    for (int e = 0; e < 4; ++e) x[e] = acc[i][j][4 * r + e];
                     if (MODE == NS_POLY) {
+                        const float4 d = EARLY ? dcol[EARLY ? 4 * j + r : 0] : d_col(j, r);
+                        const float ec[4] = {ns_rest(d.x), ns_rest(d.y), ns_rest(d.z), ns_rest(d.w)};
                         const lamq_ns_f16x4 a =
                             EARLY ? A[EARLY ? 8 * i + 4 * j + r : 0] : *reinterpret_cast<const lamq_ns_f16x4*>(g.in_hi + at);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = fmaf(g.b, (float)a[e], g.c * x[e]);
-                    }
+                        for (int e = 0; e < 4; ++e) {
+                            const float whole = (float)a[e] + (row == col + e ? er : 0.0f);
+                            x[e] = fmaf(g.b, whole, g.c * NS_UNSCALE * fmaf(er + ec[e], whole, x[e]));
+                        }
+                    } else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] *= NS_UNSCALE;
                     lamq_ns_f16x4 o;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = (_Float16)x[e];
+                    for (int e = 0; e < 4; ++e) {
+                        o[e] = (_Float16)x[e];
+                        if (row == col + e) g.diag[batch * g.mp + row] = x[e];
+                    }
                     *reinterpret_cast<lamq_ns_f16x4*>(g.out + at) = o;
                     if (I != J) {
                         uint16_t* t = g.out + (batch * g.mp + col) * (int64_t)g.la + row;
@@ -411,6 +446,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
             const int m0 = I * 64 * MT + wm + 64 * h;
             if (m0 >= g.mp) break;  // uniform: past the matrix
             if constexpr (!EARLY) {
+                dx = D[m0 + lane];
 #pragma unroll
                 for (int y = 0; y < 8; ++y) {
                     H[y] = *reinterpret_cast<const lamq_ns_f16x8*>(g.in_hi + x_at(h, y));
@@ -435,8 +471,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
                 float4* t1 = tile + row * 16 + ((2 * c8 + 1) ^ (row & 15));
                 const float4 u = *t0, w = *t1;
                 float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+                const float d = __shfl(dx, row), ah = fmaf(ns_rest(d), NS_UNSCALE, g.a), al = fmaf(d, NS_UNSCALE, g.a);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = fmaf(g.a, (float)H[y][e] + (float)L[y][e], x[e] * NS_UNSCALE);
+                for (int e = 0; e < 8; ++e)
+                    x[e] = fmaf(ah, (float)H[y][e], fmaf(al, (float)L[y][e], x[e] * NS_UNSCALE));
                 if constexpr (MODE == NS_UPDATE) {
                     lamq_ns_f16x8 hv, lv;
 #pragma unroll
@@ -484,7 +522,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
 
 // A small matrix, whole: m <= 128, n <= 512. One workgroup of 16 waves holds X in LDS as float16 (what the products
 // read) and, each wave 32 columns of it, in its accumulators as float32 times 2^10 (what a X takes), A and then B in
-// LDS; from G to the result nothing else goes through memory, and all steps are one launch. 128 x 320: 100 us by the
+// LDS; from G to the result nothing else goes through memory, and all steps are one launch. The diagonals are kept where
+// LDS has room for them, up to 96 rows; with more, the rounding averages out over the rows (7e-4). 128 x 320: 100 us by the
 // products above (17 launches of about 6 us, latencies all of it), 49 us here.
 __device__ __forceinline__ int ns_f(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }  // conflict-free both ways
 __device__ __forceinline__ uint32_t ns_xat(int row, int chunk)  // 16-byte chunk of X's row in LDS
@@ -512,8 +551,9 @@ __device__ __forceinline__ void ns_load4(const float* p, float (&v)[4])
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = x[i];
 }
-// ENTRIES: G and the result an entry a lane (a tall G, whose rows are X's columns, or rows of fewer than four), else by rows.
-template <typename Elt, bool ENTRIES>
+// ENTRIES: G and the result an entry a lane (a tall G, whose rows are X's columns, or rows of fewer than four), else by
+// rows. MT: tiles of 32 rows that X has room for; up to three, the diagonals are kept.
+template <typename Elt, bool ENTRIES, int MT>
 __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ G, int64_t ld, int64_t stride,
                                                         uint16_t* __restrict__ out, int64_t ldo, int64_t so, int m, int n,
                                                         int tall, int steps, float a, float b, float c)
@@ -528,14 +568,15 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
     G += blockIdx.x * stride;
     out += blockIdx.x * so;
     const int c0 = 32 * wave + 4 * half;  // X's rows 32 i + li, columns c0 + 8 r + {0..3}
-    lamq_ns_f32x16 X[4];
+    constexpr bool EXACT = MT < NS_SMALL_M / 32;
+    lamq_ns_f32x16 X[MT];
     double ss = 0.0;
     // No load is conditional (a branch would wait for each in turn): past the matrix the address is held inside it and the
     // value left out.
     if constexpr (ENTRIES) {
         const int64_t sr = tall ? 1 : ld, sc = tall ? ld : 1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < MT; ++i) {
             const int row = 32 * i + li;
             const Elt* g = G + (row < m ? row : m - 1) * sr;
             __builtin_amdgcn_sched_barrier(0);
@@ -550,7 +591,7 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
         const int cc = 32 * wave + 4 * (lane & 7), at = cc < n - 4 ? cc : n - 4, shift = cc - at;  // past the row by `shift`
         float4* t = reinterpret_cast<float4*>(xs) + 512 * wave;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < (MT + 1) / 2; ++h) {
             __builtin_amdgcn_sched_barrier(0);
             float x[8][4];
 #pragma unroll
@@ -567,7 +608,7 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
                 t[8 * y + ((lane & 7) ^ (y & 7))] = make_float4(shift & 2 ? s2 : s0, shift & 2 ? s3 : s1, s2, s3);
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2 && 2 * h + i < MT; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int y = 32 * i + li;
@@ -580,7 +621,7 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
             X[i][v] = 32 * i + li < m && c0 + 8 * (v >> 2) + (v & 3) < n ? X[i][v] : 0.0f;
@@ -596,16 +637,18 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
     }
     const double f = ss > 0.0 ? (double)NS_SCALE / sqrt(ss) : ss;  // NaN stays
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int v = 0; v < 16; ++v) X[i][v] = (float)((double)X[i][v] * f);
     const int ti = wave >> 2, tj = wave & 3;  // this wave's tile of A and B
     const bool mine = ti < mt && tj < mt, cols = wave < nt;  // uniform
+    float* dA = reinterpret_cast<float*>(as + (NS_SMALL_M - 32) * NS_SMALL_M * 2);  // A's and B's diagonals, where A has no rows
+    float* dB = dA + NS_SMALL_M;
     for (int step = 0; step < steps; ++step) {
         asm volatile("" : "+v"(li), "+v"(half), "+v"(i16));  // addresses are formed where they are used, not kept around the loop
         if (cols)  // X as float16
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < MT; ++i)
                 if (i < mt)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
@@ -629,7 +672,11 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
             for (int r = 0; r < 4; ++r) {
                 lamq_ns_f16x4 h;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) h[e] = (_Float16)(T[4 * r + e] * NS_UNSCALE);
+                for (int e = 0; e < 4; ++e) {
+                    T[4 * r + e] *= NS_UNSCALE;
+                    h[e] = (_Float16)T[4 * r + e];
+                    if (EXACT && ti == tj && li == 8 * r + 4 * half + e) dA[32 * ti + li] = T[4 * r + e];
+                }
                 *at(r) = h;
             }
         }
@@ -645,8 +692,20 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const lamq_ns_f16x4 h = *at(r);
+                if constexpr (EXACT) {
+                    const float er = ns_rest(dA[32 * ti + li]);
+                    const float4 d = *reinterpret_cast<const float4*>(dA + 32 * tj + 8 * r + 4 * half);
+                    const float ec[4] = {ns_rest(d.x), ns_rest(d.y), ns_rest(d.z), ns_rest(d.w)};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) T[4 * r + e] = fmaf(b, (float)h[e], c * (T[4 * r + e] * NS_UNSCALE));
+                    for (int e = 0; e < 4; ++e) {
+                        const bool on = ti == tj && li == 8 * r + 4 * half + e;
+                        const float whole = (float)h[e] + (on ? er : 0.0f);
+                        T[4 * r + e] = fmaf(b, whole, c * NS_UNSCALE * fmaf(er + ec[e], whole, T[4 * r + e]));
+                        if (on) dB[32 * ti + li] = T[4 * r + e];
+                    }
+                } else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) T[4 * r + e] = fmaf(b, (float)h[e], c * (T[4 * r + e] * NS_UNSCALE));
             }
         }
         __syncthreads();  // A is read
@@ -661,9 +720,14 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
         __syncthreads();
         if (cols) {  // X = a X + B X, onto 2^10 a X
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < MT; ++i)
+                if (EXACT) {  // and F H + diag(B) (X - H), F = diag(B) - Bh's (rows from 32 mt on are never read)
+                    const float d = dB[32 * i + li], up = fmaf(a, NS_SCALE, d), dh = -(float)(_Float16)d;
 #pragma unroll
-                for (int v = 0; v < 16; ++v) X[i][v] *= a * NS_SCALE;
+                    for (int v = 0; v < 16; ++v) X[i][v] = fmaf(up, X[i][v], dh * (float)(_Float16)X[i][v]);
+                } else
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) X[i][v] *= a * NS_SCALE;
             for (int ks = 0; ks < 2 * mt; ++ks) {
                 // depth 16 ks + 8 half + {0..7} of a column: two transposing reads of four rows each
                 const int row = 16 * ks + 8 * half + (i16 >> 2), chunk = 4 * wave + 2 * (li >> 4) + ((i16 & 3) >> 1);
@@ -674,21 +738,21 @@ __global__ __launch_bounds__(1024) void ns_small_kernel(const Elt* __restrict__ 
                 const short __attribute__((ext_vector_type(8))) y = __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7);
                 const lamq_ns_f16x8 q = __builtin_bit_cast(lamq_ns_f16x8, y);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < MT; ++i)
                     if (i < mt) {
                         const lamq_ns_f16x8 p = *(lamq_ns_lds_f16x8*)(uintptr_t)(ab + ns_aat(32 * i + li, 2 * ks + half));
                         X[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q, p, X[i], 0, 0, 0);
                     }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int v = 0; v < 16; ++v) X[i][v] *= NS_UNSCALE;
         }
         __syncthreads();  // X and B are read
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = 32 * i + li, col = c0 + 8 * r;
@@ -738,7 +802,7 @@ static NSPlan ns_plan(int64_t batch, int64_t rows, int64_t cols)
     p.la = p.mp + 64;
     p.x = (size_t)batch * p.mp * p.lx * 2;
     p.aa = (size_t)batch * p.mp * p.la * 2;
-    p.total = (size_t)batch * NS_PARTS * sizeof(double) + 3 * p.x + 2 * p.aa;
+    p.total = (size_t)batch * NS_PARTS * sizeof(double) + 3 * p.x + 2 * p.aa + 2 * (size_t)batch * p.mp * sizeof(float);
     return p;
 }
 
@@ -779,8 +843,11 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
     hipStream_t st = as_stream(stream);
     const bool tall = rows > cols;
     if (p.m <= NS_SMALL_M && p.n <= NS_SMALL_N && steps > 0) {
-        hipLaunchKernelGGL((tall || p.n < 4 ? ns_small_kernel<Elt, true> : ns_small_kernel<Elt, false>), dim3((unsigned)batch), dim3(1024), 0, st, G, ld, stride, out, ldo, so, (int)p.m,
-                           (int)p.n, (int)tall, steps, a, b, c);
+        const bool entries = tall || p.n < 4, few = p.m <= 96;
+        hipLaunchKernelGGL((few ? entries ? ns_small_kernel<Elt, true, 3> : ns_small_kernel<Elt, false, 3>
+                            : entries ? ns_small_kernel<Elt, true, 4> : ns_small_kernel<Elt, false, 4>),
+                           dim3((unsigned)batch), dim3(1024), 0, st, G, ld, stride, out, ldo, so, (int)p.m, (int)p.n, (int)tall,
+                           steps, a, b, c);
         LAMQ_LAUNCH_CHECK();
         return LAMQ_OK;
     }
@@ -790,6 +857,8 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
     uint16_t* lo = reinterpret_cast<uint16_t*>(at + 2 * p.x);
     uint16_t* A = reinterpret_cast<uint16_t*>(at + 3 * p.x);
     uint16_t* Bm = reinterpret_cast<uint16_t*>(at + 3 * p.x + p.aa);
+    float* dA = reinterpret_cast<float*>(at + 3 * p.x + 2 * p.aa);
+    float* dB = dA + batch * p.mp;
     const int64_t want = cdiv(rows * cols, 4096);
     const int nparts = (int)(want < NS_PARTS ? want : NS_PARTS);
     hipLaunchKernelGGL(ns_norm_kernel<Elt>, dim3(nparts, (unsigned)batch), dim3(256), 0, st, G, rows, cols, ld, stride, parts);
@@ -838,6 +907,7 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
         y.sp = y.sq = p.mp * p.lx;
         y.K = (int)p.np;
         y.out = A;
+        y.diag = dA;
         hipLaunchKernelGGL((alone ? ns_product_kernel<NS_GRAM, 2, 4> : ns_product_kernel<NS_GRAM, 2, 2>), lower, wg, 0, st, y);
         LAMQ_LAUNCH_CHECK();
         y.p = y.q = y.in_hi = A;
@@ -845,12 +915,15 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
         y.sp = y.sq = p.mp * p.la;
         y.K = (int)p.mp;
         y.out = Bm;
+        y.in_diag = dA;
+        y.diag = dB;
         hipLaunchKernelGGL((alone ? ns_product_kernel<NS_POLY, 2, 4> : ns_product_kernel<NS_POLY, 2, 2>), lower, wg, 0, st, y);
         LAMQ_LAUNCH_CHECK();
         y.p = Bm;
         y.q = y.in_hi = hi[k & 1];
         y.ldq = p.lx;
         y.sq = p.mp * p.lx;
+        y.in_diag = dB;
         y.out = hi[1 - (k & 1)];
         if (k + 1 < steps)
             hipLaunchKernelGGL((wide ? ns_product_kernel<NS_UPDATE, 4, 3> : apart ? ns_product_kernel<NS_UPDATE, 2, 4> : ns_product_kernel<NS_UPDATE, 2, 2>), full, wg, 0,

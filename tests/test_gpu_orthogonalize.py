@@ -72,7 +72,8 @@ def reference(G, steps=5, coeffs=COEFFS):
 def rounded_as_the_kernels(G, steps=5, coeffs=COEFFS):
     """The iteration in float64 with the kernels' float16 roundings at their places: what is left between it and the
     result are float32 sums, which flip a float16 rounding here and there, and the bf16 rounding of the result (half a
-    unit at most, 0.4 of that in the root mean square), so the result's bound from it is that half unit's norm."""
+    unit at most, 0.4 of that in the root mean square), so the result's bound from it is that half unit's norm. A's and
+    B's diagonals are whole, but in matrices of 97 to 128 rows (columns of tall ones) and up to 512 columns."""
     h = lambda x: x.to(torch.float16).double()
     X = G.double()
     tall = X.shape[0] > X.shape[1]
@@ -80,10 +81,15 @@ def rounded_as_the_kernels(G, steps=5, coeffs=COEFFS):
     a, b, c = coeffs
     hi = h(X)
     lo = h(X - hi)
+    whole = not (96 < X.shape[0] <= 128 and X.shape[1] <= 512)
+    diag = lambda x: whole * x.diagonal().unsqueeze(1)
     for _ in range(steps):
-        A = h(hi @ hi.mT / 1024)
-        B = h(b * A + c * (A @ A) / 1024)
-        X = a * (hi + lo) + B @ hi / 1024
+        A0 = hi @ hi.mT / 1024
+        A, E = h(A0), diag(A0 - h(A0))
+        At = A + torch.diag(E[:, 0])
+        B0 = b * At + c * (A @ A + (E + E.mT) * At) / 1024
+        B = h(B0)
+        X = a * (hi + lo) + (B @ hi + diag(B0 - B) * hi + diag(B0) * lo) / 1024
         hi = h(X)
         lo = h(X - hi)
     return (X.mT if tall else X) / 1024
@@ -110,6 +116,21 @@ def test_against_the_definition(m, n, kind, dt):
     check(out, *reference(G))
     near = rounded_as_the_kernels(G)
     check(out, near, UB * float(near.norm()))
+
+
+@pytest.mark.parametrize("m,n", [(1, 900), (2, 480), (3, 2000), (7, 659), (659, 7), (31, 512), (96, 512), (97, 512), (96, 513),
+                                 (128, 512), (128, 513), (600, 30)])
+def test_few_rows(m, n):
+    """Where one rounding of A or B on the diagonal would move a whole singular direction."""
+    from lookatmyquant_amd import engine as E
+
+    say(f"orthogonalize {m} x {n}, few rows")
+    for kind in ("noise", "strong", "decaying"):
+        G = gradient(m, n, kind, m + 3 * n)
+        out = E.orthogonalize(G)
+        check(out, *reference(G))
+        near = rounded_as_the_kernels(G)
+        check(out, near, UB * float(near.norm()))
 
 
 @pytest.mark.parametrize("steps,coeffs", [(0, COEFFS), (1, COEFFS), (2, (1.5, -0.5, 0.0)), (12, (1.875, -1.25, 0.375))])

@@ -25,7 +25,9 @@
 // instructions; scores, dP, delta and every sum are float32, each gradient rounded once at its end. delta is a sum of
 // products with O, and where dP - delta is small beside either, O's own rounding would show in dQ and dK (two or three
 // times the rounding of the result, over sequences of a few tokens): the forward leaves what the rounding took, a second
-// bf16 part, for it.
+// bf16 part, for it. Over short sequences the roundings of P and dS stay as large as the results' own, or larger where
+// few terms cancel; up to 128 tokens, where launches and latencies set the time, P and dS go into their products as two
+// bf16 parts.
 #include "common.h"
 
 typedef __bf16 lamq_at_bf16x8 __attribute__((ext_vector_type(8)));
@@ -48,6 +50,13 @@ __device__ __forceinline__ float at_sum32(float v)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// what bf16 takes of a value, as bf16 (nothing of an infinity)
+__device__ __forceinline__ __bf16 at_second(float x)
+{
+    const float r = x - (float)(__bf16)x;
+    return (__bf16)(r == r ? r : 0.0f);
 }
 
 // the length of sequence b, 0 .. T (all T without lengths)
@@ -214,6 +223,7 @@ __device__ __forceinline__ bool ag_place(int pairs, int per, int& pair, int& rem
 // are, and the 64 products that rescale O are left out (with the exact maximum some query of 32 grows in most blocks).
 // The sums of a query's two lanes are added at the end. 4 x 32 heads x 2,048: 195 -> 162 us against the exact maximum and
 // 32 keys a step.
+template <bool TWO>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_lse_kernel(
     AtView Q, AtView K, AtView V, AtOut O, uint16_t* __restrict__ rest, float* __restrict__ lse,
     const int32_t* __restrict__ lens, int rep, int Hkv, int pairs, int Tall, float scale_log2)
@@ -311,18 +321,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
             if (hf && k0 + 32 > my_last) break;  // uniform: past this wave's queries
-            lamq_at_bf16x8 pf[2];
+            lamq_at_bf16x8 pf[2], pl[2];
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
                 const float p = __builtin_amdgcn_exp2f(fmaf(s[hf][v], scale_log2, -m));
                 sum += p;
                 pf[v >> 3][v & 7] = (__bf16)p;
+                if (TWO) pl[v >> 3][v & 7] = at_second(p);
             }
 #pragma unroll
             for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
+                for (int t = 0; t < 4; ++t) {
                     o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[hf][mi][t], pf[mi], o[t], 0, 0, 0);
+                    if (TWO) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[hf][mi][t], pl[mi], o[t], 0, 0, 0);
+                }
         }
     }
     if (myq >= T) return;
@@ -334,6 +347,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 // dQ, and per query the log-sum-exp in units of log 2 and delta for the other kernel (rows [B, H, T] of stats and
 // stats + B H T).
+template <bool TWO>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_dq_kernel(
     AtView Q, AtView K, AtView V, AtView O, AtView dO, AtOut dQ, const uint16_t* __restrict__ rest,
     const float* __restrict__ lse,
@@ -440,16 +454,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 for (int v = 0; v < 16; ++v)
                     s[v] = k0 + 32 * hf + 8 * (v >> 2) + 4 * hi + (v & 3) <= myq ? s[v] : -__builtin_inff();
             }
-            lamq_at_bf16x8 dsf[2];
+            lamq_at_bf16x8 dsf[2], dsl[2];
 #pragma unroll
-            for (int v = 0; v < 16; ++v)
-                dsf[v >> 3][v & 7] = (__bf16)(__builtin_amdgcn_exp2f(fmaf(s[v], scale_log2, -lse2)) * dp[v]);
+            for (int v = 0; v < 16; ++v) {
+                const float ds = __builtin_amdgcn_exp2f(fmaf(s[v], scale_log2, -lse2)) * dp[v];
+                dsf[v >> 3][v & 7] = (__bf16)ds;
+                if (TWO) dsl[v >> 3][v & 7] = at_second(ds);
+            }
 #pragma unroll
             for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(tb, mi, t, hf * AG_HALF), dsf[mi], acc[t],
-                                                                     0, 0, 0);
+                for (int t = 0; t < 4; ++t) {
+                    const lamq_at_bf16x8 kt = ag_tr_frag(tb, mi, t, hf * AG_HALF);
+                    acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, dsf[mi], acc[t], 0, 0, 0);
+                    if (TWO) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kt, dsl[mi], acc[t], 0, 0, 0);
+                }
         }
     }
     if (myq < T) ag_store_row(dQp + (int64_t)myq * dQ.st, acc, scale, hi);
@@ -461,6 +480,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // so with 128 keys a workgroup four sequences of 2,048 had 512 workgroups, one for every slot of the chip, the first
 // keys' with twice the mean walk: 606 us; halved walks of half the keys go out longest first and fill each other's
 // tails. The queries are walked from the last one down, so that workgroups that start together read the same blocks.
+template <bool TWO>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void attention_dkdv_kernel(
     AtView Q, AtView K, AtView V, AtView dO, AtOut dK, AtOut dV, const int32_t* __restrict__ lens,
     const float* __restrict__ stats, int64_t nstats, int rep, int Hkv, int pairs, int Tall, float scale, float scale_log2)
@@ -556,7 +576,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 s[v] = myk <= q && q < T ? s[v] : -__builtin_inff();
             }
         }
-        lamq_at_bf16x8 pf[2], dsf[2];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float4 ls4 = *reinterpret_cast<const float4*>(sl + 8 * r);
@@ -564,19 +583,27 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int v = 4 * r + e;
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[v], scale_log2, -ls[e]));
-                pf[v >> 3][v & 7] = (__bf16)p;
-                dsf[v >> 3][v & 7] = (__bf16)(p * dp[v]);
+                s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], scale_log2, -ls[e]));
+                dp[v] *= s[v];
             }
         }
 #pragma unroll
-        for (int mi = 0; mi < 2; ++mi)
+        for (int part = 0; part < (TWO ? 2 : 1); ++part) {
+            if (part) asm volatile("" : "+v"(tb));  // the transposed tiles are read again: no registers are left to keep them
+            lamq_at_bf16x8 pf[2], dsf[2];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                dv[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(tb, mi, t, AG_OPB), pf[mi], dv[t], 0, 0, 0);
-                dk[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(tb, mi, t, 0), dsf[mi], dk[t], 0, 0,
-                                                                0);
+            for (int v = 0; v < 16; ++v) {
+                pf[v >> 3][v & 7] = part ? at_second(s[v]) : (__bf16)s[v];
+                dsf[v >> 3][v & 7] = part ? at_second(dp[v]) : (__bf16)dp[v];
             }
+#pragma unroll
+            for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    dv[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(tb, mi, t, AG_OPB), pf[mi], dv[t], 0, 0, 0);
+                    dk[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ag_tr_frag(tb, mi, t, 0), dsf[mi], dk[t], 0, 0, 0);
+                }
+        }
     }
     // the two halves of the queries: the first pair of waves takes the other's dK and ends with it, the second dV
     __syncthreads();  // everyone's last block is done with
@@ -627,6 +654,11 @@ static dim3 at_grid(int64_t wgs)
     return dim3((unsigned)gx, (unsigned)cdiv(wgs, gx));
 }
 
+// P and dS in two parts where one block of queries is all there is. 45 tokens x 32 heads: 28 -> 36 us on the device, 37 us a
+// call from the host either way, and the error over that of the results' own rounding 1.46 -> 1.00 (2 to 5 tokens: up to
+// 1.97 -> 1.00); 4 x 32 heads x 2,048: 695 -> 1,102 us, 1.43 -> 1.00
+static bool at_two(int64_t T) { return T <= AG_OWN; }
+
 static AtView at_view(const lamq_heads* x) { return AtView{x->data, x->sb, x->sh, x->st}; }
 static AtOut at_out(const lamq_heads* x) { return AtOut{x->data, x->sb, x->sh, x->st}; }
 
@@ -642,7 +674,7 @@ extern "C" int lamq_attention_causal_lse_bf16(const lamq_heads* q, const lamq_he
     if (rc != LAMQ_OK) return rc;
     if (!lse || (uintptr_t)rest % 16) return LAMQ_EINVAL;
     if (B == 0 || T == 0) return LAMQ_OK;
-    hipLaunchKernelGGL(attention_lse_kernel, at_grid(cdiv(T, AG_OWN) * H * B), dim3(256), 0, as_stream(stream), at_view(q),
+    hipLaunchKernelGGL((at_two(T) ? attention_lse_kernel<true> : attention_lse_kernel<false>), at_grid(cdiv(T, AG_OWN) * H * B), dim3(256), 0, as_stream(stream), at_view(q),
                        at_view(k), at_view(v), at_out(out), rest, lse, lens, (int)(H / Hkv), (int)Hkv, (int)(B * Hkv), (int)T,
                        scale * AT_LOG2E);
     LAMQ_LAUNCH_CHECK();
@@ -677,11 +709,12 @@ extern "C" int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_h
     float* stats = reinterpret_cast<float*>(workspace);
     const int64_t nstats = B * H * T;
     hipStream_t s = as_stream(stream);
-    hipLaunchKernelGGL(attention_dq_kernel, at_grid(cdiv(T, AG_OWN) * H * B), dim3(256), 0, s, at_view(q), at_view(k),
+    const bool two = at_two(T);
+    hipLaunchKernelGGL((two ? attention_dq_kernel<true> : attention_dq_kernel<false>), at_grid(cdiv(T, AG_OWN) * H * B), dim3(256), 0, s, at_view(q), at_view(k),
                        at_view(v), at_view(out), at_view(dout), at_out(dq), rest, lse, lens, stats, nstats, (int)(H / Hkv),
                        (int)Hkv, (int)(B * Hkv), (int)T, scale, scale * AT_LOG2E);
     LAMQ_LAUNCH_CHECK();
-    hipLaunchKernelGGL(attention_dkdv_kernel, at_grid(cdiv(T, AG_KEYS) * Hkv * B), dim3(256), 0, s, at_view(q), at_view(k),
+    hipLaunchKernelGGL((two ? attention_dkdv_kernel<true> : attention_dkdv_kernel<false>), at_grid(cdiv(T, AG_KEYS) * Hkv * B), dim3(256), 0, s, at_view(q), at_view(k),
                        at_view(v), at_view(dout), at_out(dk), at_out(dv), lens, stats, nstats, (int)(H / Hkv), (int)Hkv,
                        (int)(B * Hkv), (int)T, scale, scale * AT_LOG2E);
     LAMQ_LAUNCH_CHECK();

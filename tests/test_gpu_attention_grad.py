@@ -97,6 +97,18 @@ def test_gradients_against_the_formulas(B, H, Hkv, T):
     check(ours(*x, SCALE), *reference(*x, SCALE))
 
 
+@pytest.mark.parametrize("B,H,Hkv,T", [(2, 4, 2, 2), (3, 8, 4, 5), (1, 32, 8, 45), (2, 4, 1, 128)])
+def test_short_sequences_keep_only_the_results_rounding(B, H, Hkv, T):
+    """Up to 128 tokens P and dS enter their products whole: the error is the bf16 rounding of the results, spread over
+    half a unit in the last place, u / sqrt(3) of the norm at most (u = 2^-8) and more than a thousand numbers."""
+    say(f"attention gradients, short B={B} H={H} Hkv={Hkv} T={T}")
+    for seed in range(3):
+        x = inputs(B, H, Hkv, T, 50 + seed)
+        got, (want, _) = ours(*x, SCALE), reference(*x, SCALE)
+        for nm in ("out", "dq", "dk", "dv"):
+            assert float((got[nm].double().cpu() - want[nm]).norm() / want[nm].norm()) <= U16 / math.sqrt(3), nm
+
+
 @pytest.mark.parametrize("T,lens", [(200, [200, 0, 1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 199, -3, 500]),
                                     (1, [1, 0, 1]), (64, [0, 0]), (333, [320, 333, 150])])
 def test_lengths_and_what_padding_holds(T, lens):

@@ -484,7 +484,8 @@ int lamq_attention_causal_bf16(const uint16_t* q, int64_t sqb, int64_t sqh, int6
  *         touched)
  *   lens  [B] int32 on the device, or NULL (all T): tokens past lens[b] (held to 0 .. T) are padding. Nothing is
  *         read there; their rows of out and of the gradients are zeros, their lse -inf.
- * Sums, scores and dP are float32; P and dS are rounded to bf16 as operands of the next product, each result once.
+ * Sums, scores and dP are float32; P and dS are rounded to bf16 as operands of the next product (up to T = 128 they enter
+ * it as two bf16 parts), each result once.
  * The results do not depend on scheduling. Limits as lamq_attention_causal_bf16; the backward's token strides at most
  * 16,777,215 (LAMQ_EUNSUP above).
  * ---------------------------------------------------------------------------------------------- */
@@ -508,8 +509,8 @@ int lamq_attention_causal_grad_bf16(const lamq_heads* q, const lamq_heads* k, co
  *   X = G / ||G||_F;  steps times: A = X X^T, B = b A + c A^2, X = a X + B X  (on the short side);  out = bf16(X)
  *   G     [batch][rows, cols] bf16 bits or float32, row stride ld >= cols, matrix stride `stride` (0: one for all)
  *   out   [batch][rows, cols] bf16 bits, row stride ldo >= cols, matrix stride so >= rows ldo, not overlapping G
- * A zero matrix gives zeros, one with a NaN or an infinity NaN. The products take float16 operands (X as a sum of two)
- * and float32 sums; X's singular values, which a step maps to a s + b s^3 + c s^5, must stay within 8 from any start
+ * A zero matrix gives zeros, one with a NaN or an infinity NaN. The products take float16 operands (X as a sum of two, A's
+ * and B's diagonals in float32 beside them but for 97 to 128 rows of up to 512) and float32 sums; X's singular values, which a step maps to a s + b s^3 + c s^5, must stay within 8 from any start
  * in [0, 1], or LAMQ_EINVAL. rows, cols <= 2^20, batch <= 65,535 (LAMQ_EUNSUP above). workspace: 16-byte aligned,
  * lamq_orthogonalize_workspace_size(batch, rows, cols) bytes.
  * ---------------------------------------------------------------------------------------------- */

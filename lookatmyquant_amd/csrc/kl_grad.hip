@@ -468,7 +468,8 @@ __global__ __launch_bounds__(KG_NT) void kl_grad_part_kernel(const Elt* __restri
     }
 }
 
-// workgroups a row for T rows of V logits: enough to fill the chip with a few, at least 2,048 logits each
+// workgroups a row for T rows of V logits: enough to fill the chip with a few, at least 2,048 logits each; one where there
+// is a row for every unit (151,936 bf16 words, several workgroups a row / one: 64 rows 30 / 53 us, 128 45 / 55, 255 73 / 68)
 static int kg_splits(int64_t T, int64_t V)
 {
     if (T >= KG_SPLIT) return 1;
@@ -502,9 +503,12 @@ static int kl_grad_launch(const Elt* ref, const Elt* q, int64_t T, int64_t V, in
     if (split == 1) {
         hipLaunchKernelGGL(kl_weights_kernel, dim3(1), dim3(1024), 0, st, w, T, total);
         LAMQ_LAUNCH_CHECK();
-        // 256 threads hold a row of 16 KB in registers; longer ones take 1,024 threads and most of a unit's LDS
+        // Rows up to 96 KB: 256 threads, four rows a unit in flight to cover each other's sums, what their registers do not
+        // hold read again from the caches. Longer ones, which pass the caches so: 1,024 threads and most of a unit's LDS.
+        // 2,048 rows bf16, 256 / 1,024 threads: of 32,000 words 103 / 134 us, 49,152 179 / 181, 65,536 245 / 234, 151,936
+        // 614 / 499 (on a slower box); 1,024 rows float32: 16,384 words 50 / 57, 65,536 257 / 208
         constexpr int R = sizeof(Elt) == 2 ? 4 : 2;
-        if (V <= 8 * 256 * R)
+        if (V * (int64_t)sizeof(Elt) <= 96 * 1024)
             hipLaunchKernelGGL((kl_grad_rows_kernel<Elt, 256, R, 0>), dim3((unsigned)T), dim3(256), 0, st, ref, q, V, ldr, ldq,
                                w, total, kl, kl64, grad, ldg);
         else

@@ -524,7 +524,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, RING == 
 // read) and, each wave 32 columns of it, in its accumulators as float32 times 2^10 (what a X takes), A and then B in
 // LDS; from G to the result nothing else goes through memory, and all steps are one launch. The diagonals are kept where
 // LDS has room for them, up to 96 rows; with more, the rounding averages out over the rows (7e-4). 128 x 320: 100 us by the
-// products above (17 launches of about 6 us, latencies all of it), 49 us here.
+// products above (17 launches of about 6 us, latencies all of it), 47 us here.
 __device__ __forceinline__ int ns_f(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }  // conflict-free both ways
 __device__ __forceinline__ uint32_t ns_xat(int row, int chunk)  // 16-byte chunk of X's row in LDS
 {

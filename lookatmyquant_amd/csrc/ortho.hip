@@ -893,9 +893,10 @@ static int ns_launch(const Elt* G, int64_t batch, int64_t rows, int64_t cols, in
     x.n = (int)p.n;
     x.tall = tall;
     const dim3 lower((unsigned)(tm * (tm + 1) / 2), (unsigned)batch);
-    // a ring of four stages (all of a unit's LDS) where every tile has a unit to itself, two where two tiles share one.
-    // Updates take tiles of 256 rows, a third less of X and B through LDS, where two rounds of them fill the chip (9,728 x
-    // 2,560, 760 tiles: 134 us, of 128 rows 137; 2 x 1,024 x 2,560, 160 tiles: 21.9 us, of 128 rows 19.6)
+    // A ring of four stages (all of a unit's LDS) where every tile has a unit to itself, two where two tiles share one (X X^T,
+    // four / two: 6 tiles 10.9 / 14.7 us, 72 19.2 / 29.4, 210 74 / 98, 300 56 / 46; updates: 144 tiles 18.5 / 20.6, 320 25.4 /
+    // 20.0). Updates take tiles of 256 rows, a third less of X and B through LDS, where two rounds of them fill the chip
+    // (9,728 x 2,560, 760 tiles: 134 us, of 128 rows 137; 2 x 1,024 x 2,560, 160 tiles: 21.9 us, of 128 rows 19.6)
     const int64_t tiles = (int64_t)tm * tn * batch, tall_tiles = (int64_t)((tm + 1) / 2) * tn * batch;
     const bool alone = (int64_t)lower.x * batch <= NS_CUS, wide = tall_tiles >= 2 * NS_CUS, apart = tiles <= NS_CUS;
     x.tiles_m = wide ? (tm + 1) / 2 : tm;
